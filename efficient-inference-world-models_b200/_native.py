@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_longlong, c_size_t, c_uint8, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_longlong, c_size_t, c_uint8, c_void_p
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "liboasis_b200.so")
@@ -85,6 +85,43 @@ class VaeWeights(Structure):
                 ("pred_w", c_void_p), ("pred_b", c_void_p), ("rope", c_void_p), ("ones", c_void_p)]
 
 
+DT_BF16, DT_FP16, DT_FP32 = 0, 1, 2
+MAX_AXES = 4
+
+
+class Pages(Structure):
+    """``oasis_pages_t``: the pages of a cache."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("layers", c_int), ("pages", c_int), ("kv_heads", c_int),
+                ("page_tokens", c_int), ("head_dim", c_int), ("dtype", c_int)]
+
+
+class QkNormRope(Structure):
+    """``oasis_qk_norm_rope_t``."""
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_out", c_void_p), ("k_out", c_void_p),
+                ("q_token_stride", c_longlong), ("q_head_stride", c_longlong),
+                ("k_token_stride", c_longlong), ("k_head_stride", c_longlong),
+                ("v_token_stride", c_longlong), ("v_head_stride", c_longlong),
+                ("q_out_token_stride", c_longlong), ("q_out_head_stride", c_longlong),
+                ("k_out_token_stride", c_longlong), ("k_out_head_stride", c_longlong),
+                ("tokens", c_int), ("heads", c_int), ("kv_heads", c_int), ("head_dim", c_int), ("dtype", c_int),
+                ("norm", c_int), ("interleaved", c_int), ("eps", c_float),
+                ("q_weight", c_void_p), ("k_weight", c_void_p), ("positions", c_void_p), ("positions_64", c_int),
+                ("freqs", c_void_p), ("axes", c_int), ("axis_dims", c_int * MAX_AXES),
+                ("pages", POINTER(Pages)), ("slots", c_void_p)]
+
+
+class AttnWindow(Structure):
+    """``oasis_attn_window_t``."""
+    _fields_ = [("q", c_void_p), ("out", c_void_p), ("lse", c_void_p),
+                ("q_token_stride", c_longlong), ("q_head_stride", c_longlong),
+                ("out_token_stride", c_longlong), ("out_head_stride", c_longlong),
+                ("k", c_void_p), ("v", c_void_p), ("pages", c_int), ("kv_heads", c_int), ("page_tokens", c_int),
+                ("head_dim", c_int), ("dtype", c_int), ("page_table", c_void_p), ("table_width", c_int),
+                ("kv_len", c_void_p), ("cu_q", c_void_p), ("batch", c_int), ("tokens", c_int), ("heads", c_int),
+                ("max_q", c_int), ("max_kv", c_int), ("window", c_int), ("sinks", c_int), ("frame_tokens", c_int),
+                ("scale", c_float)]
+
+
 # name -> (restype, argtypes); every symbol include/oasis_b200.h declares
 SIGNATURES = {
     "oasis_last_error": (c_char_p, []),
@@ -116,6 +153,10 @@ SIGNATURES = {
                                      c_longlong, c_float, c_float, c_int, c_void_p]),
     "oasis_ab_update": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong,
                                 c_float, c_float, c_float, c_float, c_void_p]),
+    "oasis_pages_copy": (c_int, [POINTER(Pages), POINTER(Pages), POINTER(c_int32), POINTER(c_int32), c_int,
+                                 c_void_p]),
+    "oasis_qk_norm_rope": (c_int, [POINTER(QkNormRope), c_void_p]),
+    "oasis_attn_window": (c_int, [POINTER(AttnWindow), c_void_p]),
     "oasis_vae_workspace_size": (c_size_t, [c_int, c_int]),
     "oasis_vae_plan_create": (c_int, [POINTER(VaeWeights), c_int, c_void_p, c_size_t, POINTER(c_void_p)]),
     "oasis_vae_plan_destroy": (None, [c_void_p]),

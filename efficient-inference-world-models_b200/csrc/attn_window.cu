@@ -1,0 +1,198 @@
+// Attention over cache pages with a sliding window of frames and sink frames.
+//
+//   out = softmax(scale q K^T over the visible keys) V,  key j visible to position p iff
+//   j < kv_len, j / F <= p / F and (W == 0 or p / F - j / F < W or j / F < S).
+// The visible keys of a position are two runs: [0, sink_end) and [start, end).
+#include "launch.cuh"
+
+namespace oasis {
+
+struct WinArgs {
+  const void* q;
+  void* out;
+  float* lse;
+  long long q_ts, q_hs, o_ts, o_hs;
+  const void *k, *v;
+  int pages, kv_heads, page_tokens;
+  const int32_t* table;
+  int width;
+  const int32_t *kv_len, *cu_q;
+  int batch, tokens, heads, group;
+  int window, sinks, frame;
+  float scale_log2;  // scale * log2(e)
+};
+
+// Rows of the packed queries and cached tokens of sequence b, clamped to what exists.
+struct WinSeq {
+  int q0, n_q, kv;
+};
+__device__ __forceinline__ WinSeq win_seq(const WinArgs& a, int b) {
+  WinSeq s;
+  s.q0 = a.cu_q ? a.cu_q[b] : b;
+  int q1 = a.cu_q ? a.cu_q[b + 1] : b + 1;
+  s.q0 = max(0, min(s.q0, a.tokens));
+  q1 = max(s.q0, min(q1, a.tokens));
+  s.n_q = q1 - s.q0;
+  s.kv = max(0, min(a.kv_len[b], a.width * a.page_tokens));
+  return s;
+}
+
+struct WinRange {
+  int sink_end, start, end;  // visible: [0, sink_end) and [start, end); sink_end <= start
+  __device__ __forceinline__ bool sees(int key) const {
+    return key < end && (key >= start || key < sink_end);
+  }
+};
+__device__ __forceinline__ WinRange win_range(const WinArgs& a, int pos, int kv) {
+  WinRange r = {0, 0, 0};
+  if (pos < 0) return r;  // more queries than cached tokens
+  const int f = pos / a.frame;
+  r.end = static_cast<int>(min(static_cast<long long>(f + 1) * a.frame, static_cast<long long>(kv)));
+  if (a.window && f >= a.window) {
+    r.start = (f - a.window + 1) * a.frame;
+    r.sink_end = static_cast<int>(min(static_cast<long long>(a.sinks) * a.frame, static_cast<long long>(r.start)));
+  }
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_float(T x);
+template <>
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_float(float x) { return __float2half_rn(x); }
+
+// One query row by one warp, key after key with the running maximum and sum: each lane holds
+// D / 32 dims.  Reads only what the row sees.
+template <typename T, int D>
+__device__ void window_row(const WinArgs& a, int b, const WinSeq& s, int qi, int head, int lane) {
+  constexpr int E = D / 32;
+  const long long row = s.q0 + qi;
+  const T* q = static_cast<const T*>(a.q) + row * a.q_ts + head * a.q_hs + lane * E;
+  const WinRange r = win_range(a, s.kv - s.n_q + qi, s.kv);
+  const int kvh = head / a.group;
+  const int32_t* table = a.table + static_cast<long long>(b) * a.width;
+  float qv[E], o[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    qv[i] = to_float(q[i]) * a.scale_log2;
+    o[i] = 0.0f;
+  }
+  float m = -INFINITY, l = 0.0f;
+#pragma unroll 1
+  for (int part = 0; part < 2; ++part) {
+    const int hi = part ? r.end : r.sink_end;
+#pragma unroll 1
+    for (int key = part ? r.start : 0; key < hi; ++key) {
+      const int page = table[key / a.page_tokens];
+      if (page < 0 || page >= a.pages) continue;
+      const long long off =
+          ((static_cast<long long>(page) * a.kv_heads + kvh) * a.page_tokens + key % a.page_tokens) * D + lane * E;
+      const T* k = static_cast<const T*>(a.k) + off;
+      const T* v = static_cast<const T*>(a.v) + off;
+      float d = 0.0f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) d = fmaf(qv[i], to_float(k[i]), d);
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
+      const float mn = fmaxf(m, d);
+      const float base = mn == -INFINITY ? 0.0f : mn;
+      const float al = exp2f(m - base), p = exp2f(d - base);
+      m = mn;
+      l = l * al + p;
+#pragma unroll
+      for (int i = 0; i < E; ++i) o[i] = fmaf(p, to_float(v[i]), o[i] * al);
+    }
+  }
+  T* out = static_cast<T*>(a.out) + row * a.o_ts + head * a.o_hs + lane * E;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int i = 0; i < E; ++i) out[i] = from_float<T>(l == 0.0f ? 0.0f : o[i] * inv);
+  if (a.lse && lane == 0)
+    a.lse[row * a.heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(128) attn_window_rows_kernel(const __grid_constant__ WinArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.z, lane = threadIdx.x & 31;
+  const WinSeq s = win_seq(a, b);
+  for (int qi = blockIdx.x * 4 + (threadIdx.x >> 5); qi < s.n_q; qi += gridDim.x * 4)
+    window_row<T, D>(a, b, s, qi, blockIdx.y, lane);
+}
+
+template <typename T, int D>
+int launch_attn_window(const WinArgs& a, int max_q, int max_kv, cudaStream_t stream) {
+  cudaError_t e = launch_pdl(attn_window_rows_kernel<T, D>, dim3((max_q + 3) / 4, a.heads, a.batch), dim3(128), 0,
+                             stream, a);
+  if (e != cudaSuccess) return cuda_status(e, "attn_window_rows_kernel");
+  return OASIS_OK;
+}
+
+}  // namespace oasis
+
+extern "C" int oasis_attn_window(const oasis_attn_window_t* p, cudaStream_t stream) {
+  using namespace oasis;
+  const char* who = "oasis_attn_window";
+  if (!p) return fail(OASIS_ERR_INVALID_ARG, std::string(who) + ": null arguments");
+  if (p->batch < 0 || p->tokens < 0 || p->heads <= 0 || p->kv_heads <= 0 || p->table_width <= 0 ||
+      p->max_q < 0 || p->max_kv < 0)
+    return fail(OASIS_ERR_INVALID_ARG, std::string(who) + ": bad sizes");
+  if (p->heads % p->kv_heads)
+    return fail(OASIS_ERR_INVALID_ARG, std::string(who) + ": heads must be a multiple of kv_heads");
+  if (p->window < 0 || p->sinks < 0 || p->frame_tokens <= 0)
+    return fail(OASIS_ERR_INVALID_ARG, std::string(who) + ": window and sinks >= 0, frame_tokens >= 1");
+  if (p->head_dim != 64 && p->head_dim != 128)
+    return fail(OASIS_ERR_UNSUPPORTED, std::string(who) + ": head_dim must be 64 or 128");
+  if (p->page_tokens % 16)
+    return fail(OASIS_ERR_UNSUPPORTED, std::string(who) + ": page_tokens must be a multiple of 16");
+  if (p->dtype != OASIS_DT_BF16 && p->dtype != OASIS_DT_FP16)
+    return fail(OASIS_ERR_UNSUPPORTED, std::string(who) + ": bf16 or fp16");
+  if (!(p->scale > 0.0f) || p->scale > 3.0e38f)
+    return fail(OASIS_ERR_INVALID_ARG, std::string(who) + ": scale must be positive and finite");
+  if (p->batch > 65535 || p->heads > 65535)
+    return fail(OASIS_ERR_UNSUPPORTED, std::string(who) + ": at most 65535 sequences and heads");
+  if (static_cast<long long>(p->table_width) * p->page_tokens > 0x3fffffffLL)
+    return fail(OASIS_ERR_UNSUPPORTED, std::string(who) + ": at most 2^30 - 1 tokens per sequence");
+  if (!p->cu_q && p->tokens != p->batch)
+    return fail(OASIS_ERR_INVALID_ARG, std::string(who) + ": without cu_q there is one query per sequence");
+  if (p->batch == 0 || p->tokens == 0) return OASIS_OK;
+  if (!p->q || !p->out || !p->page_table || !p->kv_len)
+    return fail(OASIS_ERR_INVALID_ARG, std::string(who) + ": null pointer");
+  const oasis_pages_t pages = {const_cast<void*>(p->k), const_cast<void*>(p->v), 1, p->pages, p->kv_heads,
+                               p->page_tokens, p->head_dim, p->dtype};
+  if (int st = pages_check(&pages, who)) return st;
+  for (long long s : {p->q_token_stride, p->q_head_stride, p->out_token_stride, p->out_head_stride})
+    if (s % 8) return fail(OASIS_ERR_ALIGNMENT, std::string(who) + ": strides must be multiples of 16 bytes");
+  if (!aligned16(p->q) || !aligned16(p->out))
+    return fail(OASIS_ERR_ALIGNMENT, std::string(who) + ": bases must be 16-byte aligned");
+  WinArgs a = {};
+  a.q = p->q, a.out = p->out, a.lse = p->lse;
+  a.q_ts = p->q_token_stride, a.q_hs = p->q_head_stride;
+  a.o_ts = p->out_token_stride, a.o_hs = p->out_head_stride;
+  a.k = p->k, a.v = p->v;
+  a.pages = p->pages, a.kv_heads = p->kv_heads, a.page_tokens = p->page_tokens;
+  a.table = p->page_table, a.width = p->table_width;
+  a.kv_len = p->kv_len, a.cu_q = p->cu_q;
+  a.batch = p->batch, a.tokens = p->tokens, a.heads = p->heads, a.group = p->heads / p->kv_heads;
+  // a frame longer than any sequence is one frame; more sinks than any sequence are all of it
+  a.frame = std::min(p->frame_tokens, 0x3fffffff);
+  a.window = p->window;
+  a.sinks = p->sinks;
+  a.scale_log2 = p->scale * 1.4426950408889634f;
+  const int capacity = p->table_width * p->page_tokens;
+  const int max_q = !p->cu_q ? 1 : p->max_q > 0 ? std::min(p->max_q, p->tokens) : p->tokens;
+  const int max_kv = p->max_kv > 0 ? std::min(p->max_kv, capacity) : capacity;
+  if (p->dtype == OASIS_DT_BF16)
+    return p->head_dim == 64 ? launch_attn_window<__nv_bfloat16, 64>(a, max_q, max_kv, stream)
+                             : launch_attn_window<__nv_bfloat16, 128>(a, max_q, max_kv, stream);
+  return p->head_dim == 64 ? launch_attn_window<__half, 64>(a, max_q, max_kv, stream)
+                           : launch_attn_window<__half, 128>(a, max_q, max_kv, stream);
+}

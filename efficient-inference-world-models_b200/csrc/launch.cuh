@@ -38,6 +38,9 @@ int validate_slots(const oasis_kv_cache_t* c, int slot0, int frames);
 
 int num_sms();
 
+// Argument checks shared by the operators on cache pages.
+int pages_check(const oasis_pages_t* p, const char* who);
+
 int launch_attn_spatial(const void* qkv, void* out, int frames, cudaStream_t stream);
 int launch_attn_temporal(const void* qkv, const KvView& kv, int layer, void* out, int batch,
                          int q_frames, int q_pos0, int n_past, int n_kv, cudaStream_t stream);

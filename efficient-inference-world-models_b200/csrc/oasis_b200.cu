@@ -7,4 +7,7 @@
 #include "elementwise.cu"
 #include "forward.cu"
 #include "vae.cu"
+#include "paged.cu"
+#include "qk_rope.cu"
+#include "attn_window.cu"
 #include "noalloc.cu"

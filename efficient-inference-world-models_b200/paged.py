@@ -1,0 +1,650 @@
+"""Paged K/V cache and the operators on it, for streams longer than the 32-frame window, for
+sessions that branch, and for any head layout.
+
+Functions over plain tensors (each one call into ``liboasis_b200.so`` on the current stream):
+
+* :func:`qk_norm_rope`, :func:`qk_norm_rope_append` - RMS norm of every query and key head and
+  the rotation over several position axes (time, height, width) in one pass; the second also
+  writes keys and values into cache pages.
+* :func:`attn_window` - attention of packed queries over cache pages with a sliding window of
+  frames and a few sink frames that stay visible (``frame_tokens=1``: the token-wise form).
+* :func:`copy_pages` - page copies for every layer, keys and values, in one launch.
+
+:class:`PagedKVCacheB200` keeps the pages and their book: sessions own lists of pages, forks share
+pages until one of them writes (copy on write), eviction frees what the window has left behind,
+compaction moves the used pages to the front.  :class:`PagedBatchB200` is one step's plan.
+
+The operators compute results only (no gradients): inputs that require gradients are refused.
+The reference keeps whole tensors per session and concatenates each new frame
+(``kv_cache/manager.py:246-306``, ``:416-480``) and branches by copying all of it
+(``snapshot``/``restore``, ``:555-588``).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+import weakref
+from typing import Dict, List, Optional, Sequence, Tuple, Union
+
+import numpy as np
+import torch
+
+from . import _native as N
+from .kv_cache import HEAD_DIM, HEADS
+
+_DTYPES = {torch.bfloat16: N.DT_BF16, torch.float16: N.DT_FP16, torch.float32: N.DT_FP32}
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+
+def _current_stream(device_index: int) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(device_index)
+    return torch.cuda.current_stream(device_index).cuda_stream
+
+
+def _elsewhere(device: torch.device, stream) -> Optional[object]:
+    """The context a call has to be made in: another stream than the current one, or another
+    device; None where the current ones are meant."""
+    if device.type != "cuda":
+        return None
+    if stream is not None:
+        if stream.device != device:
+            raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+        return torch.cuda.stream(stream)
+    if device.index != torch.cuda.current_device():
+        return torch.cuda.device(device)
+    return None
+
+
+def _cuda(name: str, t: torch.Tensor, device: Optional[torch.device] = None) -> None:
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the queries on {device}")
+
+
+def _heads3(name: str, t: torch.Tensor) -> None:
+    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise ValueError(f"{name} must be [tokens][heads][head_dim] with contiguous head_dim")
+
+
+def _no_grad(*tensors) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("no gradient is computed here: detach the inputs or use torch.no_grad()")
+
+
+def _index32(name: str, t: torch.Tensor, shape, device) -> None:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}")
+    _cuda(name, t, device)
+
+
+def _pages(k: torch.Tensor, v: torch.Tensor, dims: Sequence[int]) -> None:
+    if k.dim() not in dims or k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError("k_pages and v_pages must be alike, [(layers)][pages][kv_heads][page_tokens][head_dim]")
+    if k.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("cache pages are bf16 or fp16")
+    if not (k.is_contiguous() and v.is_contiguous()):
+        raise ValueError("cache pages must be contiguous")
+
+
+def rope_axis_freqs(axes: Sequence[int], theta: Union[float, Sequence[float]] = 10000.0,
+                    device="cuda") -> torch.Tensor:
+    """fp64 angular frequencies of every rotated pair: axis ``a`` of ``d = axes[a]`` dims has
+    the ``d / 2`` frequencies ``theta ** (-2 i / d)`` (``theta`` may be one per axis)."""
+    thetas = [float(theta)] * len(axes) if isinstance(theta, (int, float)) else [float(t) for t in theta]
+    if len(thetas) != len(axes):
+        raise ValueError("one theta per axis")
+    if not axes or any(d <= 0 or d % 2 for d in axes) or any(not t > 0 for t in thetas):
+        raise ValueError("axes are even numbers of dims, theta is positive")
+    parts = [t ** (-2.0 * np.arange(d // 2) / d) for d, t in zip(axes, thetas)]
+    return torch.from_numpy(np.concatenate(parts)).to(device)
+
+
+def _rope_call(q, k, v, positions, freqs, q_out, k_out, pages, slots, q_weight, k_weight, axes,
+               interleaved, norm, eps) -> None:
+    dev = q.device
+    tokens, heads, d = q.shape
+    kv_heads = k.shape[1]
+    if k.shape[0] != tokens or k.shape[2] != d or k.dtype != q.dtype:
+        raise ValueError("q and k must agree in tokens, head_dim and type")
+    dt = _DTYPES.get(q.dtype)
+    if dt is None:
+        raise ValueError("q and k must be bf16, fp16 or fp32")
+    _cuda("k", k, dev)
+    n_axes = len(axes)
+    if not 1 <= n_axes <= N.MAX_AXES:
+        raise ValueError("1 to 4 position axes")
+    if positions.dim() == 1 and n_axes == 1:
+        positions = positions.unsqueeze(1)
+    if (positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (tokens, n_axes)
+            or not positions.is_contiguous()):
+        raise ValueError(f"positions must be contiguous int32 or int64 [{tokens}][{n_axes}]")
+    _cuda("positions", positions, dev)
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or 2 * freqs.shape[0] != sum(axes) or not freqs.is_contiguous():
+        raise ValueError("freqs must be a contiguous fp64 tensor of sum(axes) / 2 frequencies")
+    _cuda("freqs", freqs, dev)
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            if not norm:
+                raise ValueError(f"{name} without the norm")
+            if w.dtype != torch.float32 or tuple(w.shape) != (d,) or not w.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous fp32 tensor [{d}]")
+            _cuda(name, w, dev)
+    _no_grad(q, k, v, q_weight, k_weight)
+    qs, ks, qos = q.stride(), k.stride(), q_out.stride()
+    vs = v.stride() if v is not None else (0, 0)
+    kos = k_out.stride() if k_out is not None else (0, 0)
+    args = N.QkNormRope(
+        q.data_ptr(), k.data_ptr(), v.data_ptr() if v is not None else None, q_out.data_ptr(),
+        k_out.data_ptr() if k_out is not None else None, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], qos[0], qos[1],
+        kos[0], kos[1], tokens, heads, kv_heads, d, dt, norm, interleaved, eps,
+        q_weight.data_ptr() if q_weight is not None else None,
+        k_weight.data_ptr() if k_weight is not None else None, positions.data_ptr(),
+        positions.dtype == torch.int64, freqs.data_ptr(), n_axes, tuple(axes),
+        ctypes.pointer(pages) if pages is not None else None, slots.data_ptr() if slots is not None else None)
+    N.check(N.lib().oasis_qk_norm_rope(args, _current_stream(dev.index)))
+
+
+def _rope_out(name: str, out: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+        raise ValueError(f"{name} must have its input's shape, type and device")
+    _heads3(name, out)
+    if out.data_ptr() == like.data_ptr() and out.stride() != like.stride():
+        raise ValueError(f"{name} over its input must have the input's strides")
+    return out
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *,
+                 axes: Sequence[int], interleaved: bool = True, norm: bool = True,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                 eps: float = 1e-6, q_out: Optional[torch.Tensor] = None,
+                 k_out: Optional[torch.Tensor] = None, stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Per-head RMS norm (unless ``norm=False``) and rotation of q [tokens][heads][head_dim] and
+    k [tokens][kv_heads][head_dim], bf16, fp16 or fp32, any token and head strides of 16 bytes
+    (see ``oasis_qk_norm_rope``).  ``axes`` gives the dims each position axis rotates (their sum
+    may be less than head_dim: the rest is only normed), ``positions`` [tokens][len(axes)] int32 or
+    int64, ``freqs`` the fp64 frequencies of the pairs (:func:`rope_axis_freqs`).  Pairs are
+    neighbours (``interleaved``, as the model here rotates) or halves of the rotated dims.  q_out / k_out may
+    be q / k.  Returns (q_out, k_out)."""
+    _heads3("q", q)
+    _heads3("k", k)
+    _cuda("q", q)
+    there = _elsewhere(q.device, stream)
+    if there is not None:
+        with there:
+            return qk_norm_rope(q, k, positions, freqs, axes=axes, interleaved=interleaved, norm=norm,
+                                q_weight=q_weight, k_weight=k_weight, eps=eps, q_out=q_out, k_out=k_out)
+    q_out, k_out = _rope_out("q_out", q_out, q), _rope_out("k_out", k_out, k)
+    _rope_call(q, k, None, positions, freqs, q_out, k_out, None, None, q_weight, k_weight, axes, interleaved,
+               norm, eps)
+    return q_out, k_out
+
+
+def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                        freqs: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                        slots: torch.Tensor, *, axes: Sequence[int], interleaved: bool = True,
+                        norm: bool = True, q_weight: Optional[torch.Tensor] = None,
+                        k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                        q_out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """:func:`qk_norm_rope` whose keys go, with the values v [tokens][kv_heads][head_dim], into
+    cache pages [pages][kv_heads][page_tokens][head_dim]: token i into slot ``slots[i] = page *
+    page_tokens + offset`` (int32; a token whose slot lies outside the pages, such as -1, is not stored;
+    slots are distinct).  Returns q_out."""
+    _heads3("q", q)
+    _heads3("k", k)
+    _heads3("v", v)
+    _cuda("q", q)
+    there = _elsewhere(q.device, stream)
+    if there is not None:
+        with there:
+            return qk_norm_rope_append(q, k, v, positions, freqs, k_pages, v_pages, slots, axes=axes,
+                                       interleaved=interleaved, norm=norm, q_weight=q_weight,
+                                       k_weight=k_weight, eps=eps, q_out=q_out)
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError("v must have k's shape and type")
+    _cuda("v", v, q.device)
+    _pages(k_pages, v_pages, (4,))
+    _cuda("k_pages", k_pages, q.device)
+    _cuda("v_pages", v_pages, q.device)
+    n_pages, kv_heads, page_tokens, d = k_pages.shape
+    if kv_heads != k.shape[1] or d != k.shape[2] or k_pages.dtype != k.dtype:
+        raise ValueError("the pages do not fit the keys (kv_heads, head_dim, type)")
+    _index32("slots", slots, (q.shape[0],), q.device)
+    q_out = _rope_out("q_out", q_out, q)
+    pages = N.Pages(k_pages.data_ptr(), v_pages.data_ptr(), 1, n_pages, kv_heads, page_tokens, d,
+                    _DTYPES[k_pages.dtype])
+    _rope_call(q, k, v, positions, freqs, q_out, None, pages, slots, q_weight, k_weight, axes, interleaved, norm,
+               eps)
+    return q_out
+
+
+def attn_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                kv_len: torch.Tensor, cu_q: Optional[torch.Tensor] = None, *, window: Optional[int] = None,
+                sinks: int = 0, frame_tokens: int = 1, scale: Optional[float] = None,
+                max_q: Optional[int] = None, max_kv: Optional[int] = None,
+                out: Optional[torch.Tensor] = None, return_lse: bool = False, stream=None):
+    """Attention of packed queries over cache pages (see ``oasis_attn_window``).
+
+    q [tokens][heads][head_dim] bf16 or fp16, head_dim 64 or 128; k_pages / v_pages
+    [pages][kv_heads][page_tokens][head_dim], heads a multiple of kv_heads, page_tokens of 16.
+    Sequence b owns queries ``cu_q[b]:cu_q[b+1]`` (``cu_q`` None: one query each) and ``kv_len[b]``
+    cached tokens in the pages ``page_table[b]`` (an entry outside the pages, such as -1, hides its
+    tokens); its queries are the last of them.  A query of frame f (``position // frame_tokens``)
+    sees the frames up to its own that are fewer than ``window`` frames back (None: all) or among
+    the first ``sinks``.  ``scale`` defaults to head_dim ** -0.5.  A query that sees nothing gets zeros.
+
+    ``max_q`` / ``max_kv`` (bounds on the queries and tokens of a sequence) only choose the launch.
+    Rows that belong to no sequence are not written.  ``out`` may be q.  Returns out, or (out, lse)
+    with lse fp32 [tokens][heads], the natural logarithm of the softmax sum."""
+    _heads3("q", q)
+    _cuda("q", q)
+    dev = q.device
+    there = _elsewhere(dev, stream)
+    if there is not None:
+        with there:
+            return attn_window(q, k_pages, v_pages, page_table, kv_len, cu_q, window=window, sinks=sinks,
+                               frame_tokens=frame_tokens, scale=scale, max_q=max_q, max_kv=max_kv, out=out,
+                               return_lse=return_lse)
+    tokens, heads, d = q.shape
+    _pages(k_pages, v_pages, (4,))
+    _cuda("k_pages", k_pages, dev)
+    _cuda("v_pages", v_pages, dev)
+    n_pages, kv_heads, page_tokens, d2 = k_pages.shape
+    if d2 != d or k_pages.dtype != q.dtype:
+        raise ValueError("the pages do not fit the queries (head_dim, type)")
+    if page_table.dim() != 2:
+        raise ValueError("page_table must be [sequences][pages]")
+    batch, width = page_table.shape
+    _index32("page_table", page_table, (batch, width), dev)
+    _index32("kv_len", kv_len, (batch,), dev)
+    if cu_q is not None:
+        _index32("cu_q", cu_q, (batch + 1,), dev)
+    elif tokens != batch:
+        raise ValueError("without cu_q there is one query per sequence")
+    if window is not None and window < 1:
+        raise ValueError("window must be at least one frame (None: no window)")
+    if sinks < 0 or frame_tokens < 1:
+        raise ValueError("sinks must be >= 0 and frame_tokens >= 1")
+    _no_grad(q, k_pages, v_pages)
+    if out is None:
+        out = torch.empty((tokens, heads, d), dtype=q.dtype, device=dev)
+    else:
+        out = _rope_out("out", out, q)
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=dev) if return_lse else None
+    big = 0x3fffffff
+    qs, os_ = q.stride(), out.stride()
+    args = N.AttnWindow(
+        q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None, qs[0], qs[1], os_[0], os_[1],
+        k_pages.data_ptr(), v_pages.data_ptr(), n_pages, kv_heads, page_tokens, d, _DTYPES[q.dtype],
+        page_table.data_ptr(), width, kv_len.data_ptr(), cu_q.data_ptr() if cu_q is not None else None, batch, tokens,
+        heads, min(max_q or 0, big), min(max_kv or 0, big), min(window or 0, big), min(sinks, big),
+        min(frame_tokens, big), d ** -0.5 if scale is None else scale)
+    N.check(N.lib().oasis_attn_window(args, _current_stream(dev.index)))
+    return (out, lse) if return_lse else out
+
+
+_int32_p = ctypes.POINTER(ctypes.c_int32)
+
+
+def _page_list(name: str, x) -> np.ndarray:
+    if isinstance(x, torch.Tensor):
+        if x.is_cuda:
+            raise ValueError(f"{name} must be on the host: it is checked before the launch")
+        x = x.numpy()
+    x = np.asarray(x)
+    if x.size == 0:
+        x = x.astype(np.int32)
+    if x.ndim != 1 or x.dtype.kind not in "iu":
+        raise ValueError(f"{name} must be a list of page numbers")
+    if x.dtype != np.int32:
+        if x.max(initial=0) > 0x7fffffff or x.min(initial=0) < -1:
+            raise ValueError(f"{name}: page number out of range")
+        x = x.astype(np.int32)
+    return np.ascontiguousarray(x)
+
+
+def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src, dst, *, to=None, stream=None) -> None:
+    """Copy page ``src[i]`` to page ``dst[i]`` for every layer, keys and values, in one launch
+    (see ``oasis_pages_copy``).  k_pages / v_pages [(layers)][pages][kv_heads][page_tokens][head_dim];
+    ``src`` and ``dst`` are host lists (or int tensors, arrays) of page numbers, free to change once the call returns.
+    A page may be copied to several places; within one cache no destination may also be a source.  ``to``:
+    the (k, v) pages of another cache that receives the pages."""
+    _pages(k_pages, v_pages, (4, 5))
+    _cuda("k_pages", k_pages)
+    dev = k_pages.device
+    _cuda("v_pages", v_pages, dev)
+    there = _elsewhere(dev, stream)
+    if there is not None:
+        with there:
+            return copy_pages(k_pages, v_pages, src, dst, to=to)
+    k2, v2 = (k_pages, v_pages) if to is None else to
+    if to is not None:
+        _pages(k2, v2, (4, 5))
+        _cuda("to", k2, dev)
+        _cuda("to", v2, dev)
+        if (k2.dim() != k_pages.dim() or k2.dtype != k_pages.dtype or k2.shape[-3:] != k_pages.shape[-3:]
+                or k2.shape[:-4] != k_pages.shape[:-4]):
+            raise ValueError("the caches' pages differ")
+    src, dst = _page_list("src", src), _page_list("dst", dst)
+    if src.shape != dst.shape:
+        raise ValueError("src and dst must have the same length")
+    layers = k_pages.shape[0] if k_pages.dim() == 5 else 1
+    tail = (*k_pages.shape[-3:], _DTYPES[k_pages.dtype])
+    a = N.Pages(k_pages.data_ptr(), v_pages.data_ptr(), layers, k_pages.shape[-4], *tail)
+    b = a if to is None else N.Pages(k2.data_ptr(), v2.data_ptr(), layers, k2.shape[-4], *tail)
+    N.check(N.lib().oasis_pages_copy(a, b, src.ctypes.data_as(_int32_p), dst.ctypes.data_as(_int32_p), src.shape[0],
+                                     _current_stream(dev.index)))
+
+
+class PagedBatchB200:
+    """One step of some sessions: their new tokens and where those live in the cache.
+
+    ``cu_q`` int32 [n+1], ``kv_len`` int32 [n], ``page_table`` int32 [n][width], ``slots`` int32
+    [tokens]: the device arrays that :func:`attn_window` and :func:`qk_norm_rope_append` take, parts
+    of one buffer.  ``max_q``, ``max_kv`` are the launch bounds.  Rebuilt in place by
+    ``PagedKVCacheB200.step(..., into=batch)`` (the same sessions' count and tokens), so a captured
+    graph that reads it can be replayed step after step."""
+
+    def __init__(self, sequences: int, tokens: int, width: int, page_tokens: int, device):
+        self.sequences, self.tokens, self.width = sequences, tokens, width
+        self.max_kv = width * page_tokens
+        self.max_q = 0
+        self.seqs: Tuple[int, ...] = ()
+        self.stale = True
+        n = 2 * sequences + 1 + sequences * width + tokens
+        self._buffer = torch.empty(n, dtype=torch.int32, device=device)
+        cu, lens, table, slots = self._buffer.split([sequences + 1, sequences, sequences * width, tokens])
+        self.cu_q, self.kv_len, self.page_table, self.slots = cu, lens, table.view(sequences, width), slots
+
+
+class _Stream:
+    """Host record of a session: its pages in order (-1: evicted) and its tokens."""
+
+    __slots__ = ("pages", "length", "batches")
+
+    def __init__(self, pages: List[int], length: int):
+        self.pages, self.length = pages, length
+        self.batches: List[weakref.ref] = []
+
+    def changed(self) -> None:
+        """The plans made of this record no longer describe it."""
+        for r in self.batches:
+            b = r()
+            if b is not None:
+                b.stale = True
+        self.batches.clear()
+
+
+class PagedKVCacheB200:
+    """K/V pages of any number of sessions, for ``layers`` layers:
+    ``k``, ``v`` [layers][pages][kv_heads][page_tokens][head_dim].
+
+    The book is kept on the host; device work is the page copies of :meth:`step` (copy on write),
+    :meth:`compact` and :meth:`adopt`, on the current stream.  A method that raises has changed nothing."""
+
+    def __init__(self, layers: int, pages: int, page_tokens: int = 16, kv_heads: int = HEADS,
+                 head_dim: int = HEAD_DIM, dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        if min(layers, pages, page_tokens, kv_heads) < 1:
+            raise ValueError("layers, pages, page_tokens and kv_heads must be positive")
+        if page_tokens % 16 or head_dim not in (64, 128) or dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("page_tokens must be a multiple of 16, head_dim 64 or 128, dtype bf16 or fp16")
+        if pages * page_tokens > 0x7fffffff:
+            raise ValueError("more than 2^31 - 1 token slots")
+        self.layers, self.pages, self.page_tokens = layers, pages, page_tokens
+        self.kv_heads, self.head_dim, self.dtype = kv_heads, head_dim, dtype
+        shape = (layers, pages, kv_heads, page_tokens, head_dim)
+        self.k = torch.zeros(shape, dtype=dtype, device=device)
+        self.v = torch.zeros(shape, dtype=dtype, device=device)
+        self.device = self.k.device
+        self._free = list(range(pages - 1, -1, -1))
+        self._refs = [0] * pages
+        self._seqs: Dict[int, _Stream] = {}
+        self._next = 0
+
+    # -- the book ------------------------------------------------------------------------
+    def _get(self, seq: int) -> _Stream:
+        s = self._seqs.get(seq)
+        if s is None:
+            raise ValueError(f"no session {seq} in this cache")
+        return s
+
+    def _put(self, s: _Stream) -> int:
+        seq, self._next = self._next, self._next + 1
+        self._seqs[seq] = s
+        return seq
+
+    def _drop(self, page: int) -> None:
+        if page < 0:
+            return
+        self._refs[page] -= 1
+        if self._refs[page] == 0:
+            self._free.append(page)
+
+    def _take(self) -> int:
+        page = self._free.pop()
+        self._refs[page] = 1
+        return page
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    @property
+    def sessions(self) -> List[int]:
+        return list(self._seqs)
+
+    def length(self, seq: int) -> int:
+        """Tokens of a session, evicted ones included."""
+        return self._get(seq).length
+
+    def pages_of(self, seq: int) -> List[int]:
+        """The session's pages in order; -1 where evicted."""
+        return list(self._get(seq).pages)
+
+    def new(self) -> int:
+        """A new, empty session."""
+        return self._put(_Stream([], 0))
+
+    def fork(self, seq: int, copies: int = 1) -> List[int]:
+        """``copies`` new sessions that continue ``seq``: they share its pages, and whoever writes
+        into a shared page first gets a copy of it.  No device work."""
+        s = self._get(seq)
+        if copies < 0:
+            raise ValueError("copies must be >= 0")
+        for p in s.pages:
+            if p >= 0:
+                self._refs[p] += copies
+        return [self._put(_Stream(list(s.pages), s.length)) for _ in range(copies)]
+
+    def free(self, seq: int) -> None:
+        """End a session; pages that no other session shares become free."""
+        s = self._get(seq)
+        for p in s.pages:
+            self._drop(p)
+        s.changed()
+        del self._seqs[seq]
+
+    def truncate(self, seq: int, length: int) -> None:
+        """Keep the first ``length`` tokens (rejected frames go).  Evicted pages stay evicted."""
+        s = self._get(seq)
+        if not 0 <= length <= s.length:
+            raise ValueError(f"length must be 0..{s.length}")
+        keep = -(-length // self.page_tokens)
+        for p in s.pages[keep:]:
+            self._drop(p)
+        del s.pages[keep:]
+        s.length = length
+        s.changed()
+
+    def evict(self, seq: int, window: int, sinks: int = 0, frame_tokens: int = 1) -> int:
+        """Give up the pages that no later token of the session can see under this window: all
+        their tokens are before the window of the next token's frame and behind the sink frames.
+        Returns how many."""
+        s = self._get(seq)
+        if window < 1 or sinks < 0 or frame_tokens < 1:
+            raise ValueError("window and frame_tokens must be >= 1, sinks >= 0")
+        start = max(0, s.length // frame_tokens - window + 1) * frame_tokens
+        first = -(-sinks * frame_tokens // self.page_tokens)
+        gone = [i for i in range(first, start // self.page_tokens) if s.pages[i] >= 0]
+        for i in gone:
+            self._drop(s.pages[i])
+            s.pages[i] = -1
+        if gone:
+            s.changed()
+        return len(gone)
+
+    # -- device work ---------------------------------------------------------------------
+    def copy_pages(self, src, dst, stream=None) -> None:
+        """Raw page copies (the book is not touched): see :func:`copy_pages`."""
+        copy_pages(self.k, self.v, src, dst, stream=stream)
+
+    def _own(self, wants: Sequence[Tuple[_Stream, int, int]], stream) -> None:
+        """For every (session, first, length): make the pages of tokens first..length-1 exist and
+        belong to the session alone, copying shared ones that hold tokens to keep."""
+        pt = self.page_tokens
+        refs = dict()  # what the references will be: a shared page's last sharer writes in place
+        need = 0
+        plan: List[Tuple[_Stream, List[int], int]] = []
+        for s, first, length in wants:
+            shared = []
+            if first < length:
+                for i in range(first // pt, min(-(-length // pt), len(s.pages))):
+                    p = s.pages[i]
+                    if p < 0:
+                        raise ValueError("a token to be written lies in an evicted page")
+                    if refs.setdefault(p, self._refs[p]) > 1:
+                        refs[p] -= 1
+                        shared.append(i)
+            fresh = max(0, -(-length // pt) - len(s.pages))
+            need += fresh + len(shared)
+            plan.append((s, shared, fresh))
+        if need > len(self._free):
+            raise RuntimeError(f"paged KV cache: {need} pages needed, {len(self._free)} free")
+        src, dst = [], []
+        for s, shared, fresh in plan:
+            for i in shared:
+                old, s.pages[i] = s.pages[i], self._take()
+                src.append(old)
+                dst.append(s.pages[i])
+                self._drop(old)
+            s.pages.extend(self._take() for _ in range(fresh))
+            if shared or fresh:
+                s.changed()
+        if src:
+            self.copy_pages(src, dst, stream)
+
+    def step(self, seqs: Sequence[int], tokens: Union[int, Sequence[int]], *, extend: bool = True,
+             table_width: Optional[int] = None, into: Optional[PagedBatchB200] = None,
+             stream=None) -> PagedBatchB200:
+        """The plan of one step: ``tokens`` new tokens for each session (one number or one each).
+        With ``extend=False`` the step's tokens are the sessions' last ones again (the same frame
+        at another solver step: its keys and values are written anew).  Pages are taken, and
+        shared ones that the step writes into are copied first.  ``table_width``: pages per session
+        the plan has room for (default: what this step needs).  ``into``: rebuild this plan in place, on the current
+        stream, for the same number of sessions and tokens."""
+        seqs = [int(i) for i in seqs]
+        if not seqs or len(set(seqs)) != len(seqs):
+            raise ValueError("a step takes one or more different sessions")
+        counts = [int(tokens)] * len(seqs) if isinstance(tokens, (int, np.integer)) else [int(t) for t in tokens]
+        if len(counts) != len(seqs) or min(counts) < 0:
+            raise ValueError("one token count >= 0 per session")
+        streams = [self._get(i) for i in seqs]
+        lengths = [s.length + (n if extend else 0) for s, n in zip(streams, counts)]
+        if any(n > m for n, m in zip(counts, lengths)):
+            raise ValueError("a session has fewer tokens than the step rewrites")
+        pt, total = self.page_tokens, sum(counts)
+        need = max(1, max(-(-m // pt) for m in lengths))
+        width = into.width if into is not None else max(need, table_width or 0)
+        if need > width:
+            raise ValueError(f"the plan has room for {width} pages per session, {need} are needed")
+        if into is not None and (into.sequences != len(seqs) or into.tokens != total):
+            raise ValueError(f"the plan is for {into.sequences} sessions and {into.tokens} tokens")
+        if width * pt > 0x3fffffff:
+            raise ValueError("more than 2^30 - 1 tokens in a session")
+        self._own([(s, m - n, m) for s, n, m in zip(streams, counts, lengths)], stream)
+        for s, m in zip(streams, lengths):
+            if m != s.length:
+                s.length = m
+                s.changed()
+        n = len(seqs)
+        host = np.full(2 * n + 1 + n * width + total, -1, np.int32)
+        cu = host[: n + 1]
+        cu[0] = 0
+        np.cumsum(counts, out=cu[1:])
+        host[n + 1: 2 * n + 1] = lengths
+        table = host[2 * n + 1: 2 * n + 1 + n * width].reshape(n, width)
+        slots = host[2 * n + 1 + n * width:]
+        for i, (s, c, m) in enumerate(zip(streams, counts, lengths)):
+            table[i, : len(s.pages)] = s.pages
+            at = np.arange(m - c, m)
+            slots[cu[i]: cu[i + 1]] = table[i, at // pt].astype(np.int64) * pt + at % pt
+        b = into if into is not None else PagedBatchB200(n, total, width, pt, self.device)
+        there = _elsewhere(self.device, stream)
+        if there is not None:
+            with there:
+                b._buffer.copy_(torch.from_numpy(host))
+        else:
+            b._buffer.copy_(torch.from_numpy(host))
+        b.max_q = max(max(counts), b.max_q)  # a captured launch keeps the bound it was captured with
+        for i in b.seqs:  # a rebuilt plan no longer follows its earlier sessions
+            old = self._seqs.get(i)
+            if old is not None:
+                old.batches = [r for r in old.batches if r() is not b]
+        b.seqs, b.stale = tuple(seqs), False
+        for s in streams:
+            s.batches = [r for r in s.batches if r() is not None] + [weakref.ref(b)]
+        return b
+
+    def compact(self, stream=None) -> int:
+        """Move the used pages to the front of the pools (one launch) and return their number."""
+        used = self.pages - len(self._free)
+        src = [p for p in range(used, self.pages) if self._refs[p]]
+        dst = [p for p in range(used) if not self._refs[p]]
+        if src:
+            self.copy_pages(src, dst, stream)
+            to = dict(zip(src, dst))
+            for s in self._seqs.values():
+                s.pages = [to.get(p, p) for p in s.pages]
+                s.changed()
+            for p, n in to.items():
+                self._refs[n], self._refs[p] = self._refs[p], 0
+        self._free = list(range(self.pages - 1, used - 1, -1))
+        return used
+
+    def adopt(self, other: "PagedKVCacheB200", seq: int, stream=None) -> int:
+        """A session of another cache (of the same layers, heads, page size and type) continues here:
+        its pages are copied, sharing is not kept.  Returns its number here; the other keeps its own."""
+        if other is self:
+            raise ValueError("adopt takes a session of another cache: fork one of this")
+        s = other._get(seq)
+        held = [p for p in s.pages if p >= 0]
+        if len(held) > len(self._free):
+            raise RuntimeError(f"paged KV cache: {len(held)} pages needed, {len(self._free)} free")
+        dst = self._free[len(self._free) - len(held):][::-1]
+        if held:
+            copy_pages(other.k, other.v, held, dst, to=(self.k, self.v), stream=stream)
+        taken = iter([self._take() for _ in held])
+        return self._put(_Stream([next(taken) if p >= 0 else -1 for p in s.pages], s.length))
+
+    # -- a layer's operators on a step -----------------------------------------------------
+    def _live(self, batch: PagedBatchB200) -> None:
+        if batch.stale:
+            raise ValueError("the step's plan is out of date: its sessions' pages have changed since")
+
+    def append(self, layer: int, batch: PagedBatchB200, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+               positions: torch.Tensor, freqs: torch.Tensor, **kw) -> torch.Tensor:
+        """:func:`qk_norm_rope_append` of the step's tokens into this layer's pages."""
+        self._live(batch)
+        return qk_norm_rope_append(q, k, v, positions, freqs, self.k[layer], self.v[layer], batch.slots, **kw)
+
+    def attend(self, layer: int, batch: PagedBatchB200, q: torch.Tensor, **kw):
+        """:func:`attn_window` of the step's queries over this layer's pages."""
+        self._live(batch)
+        return attn_window(q, self.k[layer], self.v[layer], batch.page_table, batch.kv_len, batch.cu_q,
+                           max_q=max(1, batch.max_q), max_kv=batch.max_kv, **kw)

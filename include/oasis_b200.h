@@ -335,6 +335,89 @@ void oasis_vae_plan_destroy(oasis_vae_plan_t* plan);
  * Enqueues on `stream`, allocates nothing; one decode per plan at a time. */
 int oasis_vae_decode(oasis_vae_plan_t* plan, const float* z, float* out, cudaStream_t stream);
 
+/* ------------------------------------------------------------------ paged cache */
+/* Operators on a cache of fixed-size pages, for streams longer than the OASIS_MAX_FRAMES
+ * window and for any head layout.  A token stream (a session) owns a list of pages; pages
+ * may be shared by several streams (forks).  The reference keeps whole tensors per session
+ * and concatenates (kv_cache/manager.py:246-306,416-480). */
+#define OASIS_DT_BF16 0
+#define OASIS_DT_FP16 1
+#define OASIS_DT_FP32 2
+
+/* Pages of a cache: k and v each [layers][pages][kv_heads][page_tokens][head_dim] of
+ * `dtype`, contiguous, 16-byte aligned. */
+typedef struct {
+  void* k; void* v;
+  int layers, pages, kv_heads, page_tokens, head_dim, dtype;
+} oasis_pages_t;
+
+/* Copies page src_pages[i] of `src` into page dst_pages[i] of `dst`, for every layer, keys
+ * and values, 0 <= i < n.  The lists are HOST memory, read during the call.  `src` and
+ * `dst` may be the same cache (then no destination page may also be a source page); they
+ * must agree in everything but `pages`.  A source may be listed several times, a
+ * destination once.  Used for the copy-on-write of forked sessions, for compaction, and to
+ * hand sessions over to another cache. */
+int oasis_pages_copy(const oasis_pages_t* src, const oasis_pages_t* dst, const int32_t* src_pages,
+                     const int32_t* dst_pages, int n, cudaStream_t stream);
+
+/* Norm of every query and key head and rotation over up to OASIS_MAX_AXES position axes,
+ * in one pass over tokens [0, tokens):
+ *   y = norm ? x * rsqrt(mean(x^2) + eps) * weight : x          (statistics in fp32)
+ *   pair p < sum(axis_dims)/2 of y: (a, b) -> (a cos - b sin, b cos + a sin) with the angle
+ *   positions[token][axis of p] * freqs[p], reduced in fp64; the other dims pass through.
+ * Pair p is dims (2p, 2p+1) if `interleaved`, else (p, p + rot/2) with rot = sum(axis_dims);
+ * axis a owns axis_dims[a]/2 consecutive pairs.
+ * Strides are in elements; the head_dim elements of a head are contiguous.  Bases are 16-byte
+ * aligned, strides multiples of 16 bytes.  q_out may be q and k_out may be k (same strides).
+ * With `pages` (one layer: the slice of it) k and v of token i go into slot slots[i] = page *
+ * page_tokens + offset instead of k_out; tokens whose slot is outside the pages are not stored.
+ * head_dim 32, 64, 128 or 256; the half-split form needs rot % 16 == 0. */
+#define OASIS_MAX_AXES 4
+typedef struct {
+  const void* q; const void* k; const void* v;
+  void* q_out; void* k_out;
+  long long q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+  long long v_token_stride, v_head_stride;
+  long long q_out_token_stride, q_out_head_stride, k_out_token_stride, k_out_head_stride;
+  int tokens, heads, kv_heads, head_dim, dtype;
+  int norm, interleaved;
+  float eps;
+  const float* q_weight; const float* k_weight;   /* fp32 [head_dim] or NULL (ones)        */
+  const void* positions; int positions_64;        /* [tokens][axes], int32 or int64        */
+  const double* freqs;                            /* fp64 [sum(axis_dims)/2], radians      */
+  int axes; int axis_dims[OASIS_MAX_AXES];
+  const oasis_pages_t* pages; const int32_t* slots;
+} oasis_qk_norm_rope_t;
+int oasis_qk_norm_rope(const oasis_qk_norm_rope_t* args, cudaStream_t stream);
+
+/* Attention of packed queries over cache pages with a sliding window of frames and sink
+ * frames.  Sequence b has queries cu_q[b]..cu_q[b+1]-1 of `q` [tokens][heads][head_dim]
+ * (cu_q NULL: query b alone) and kv_len[b] cached tokens, its queries' own included: query i
+ * of n stands at position kv_len[b] - n + i.  Key j is visible to the query at position p iff
+ *   j < kv_len[b]  and  j / F <= p / F  and
+ *   (window == 0  or  p / F - j / F < window  or  j / F < sinks),     F = frame_tokens,
+ * so frames see themselves whole, and F = 1 is the token-wise causal form.  Key j lies in page
+ * page_table[b][j / page_tokens]; the tokens of an entry outside [0, pages) are not visible.
+ * A query that sees nothing gets zeros (lse: -inf).  Rows outside every sequence are not
+ * written.  out may be q (same strides).  lse (may be NULL): fp32 [tokens][heads], natural
+ * logarithm.  Keys and values that a query does not see do not reach its result, whatever
+ * they hold.
+ * heads % kv_heads == 0; head_dim 64 or 128; page_tokens % 16 == 0; bf16 or fp16.
+ * max_q and max_kv are bounds for choosing the launch (0: from the shapes); they do not
+ * change the result. */
+typedef struct {
+  const void* q; void* out; float* lse;
+  long long q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  const void* k; const void* v;                  /* [pages][kv_heads][page_tokens][head_dim] */
+  int pages, kv_heads, page_tokens, head_dim, dtype;
+  const int32_t* page_table; int table_width;    /* [batch][table_width]                  */
+  const int32_t* kv_len; const int32_t* cu_q;
+  int batch, tokens, heads, max_q, max_kv;
+  int window, sinks, frame_tokens;
+  float scale;
+} oasis_attn_window_t;
+int oasis_attn_window(const oasis_attn_window_t* args, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,284 @@
+"""Host side of the paged cache: the book of pages (on CPU tensors, where no kernel runs) and the
+C entry points' refusals (checked before any launch)."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+P = ctypes.c_void_p
+
+
+def make(pkg, pages=12, layers=2, **kw):
+    c = pkg.PagedKVCacheB200(layers, pages, page_tokens=16, kv_heads=2, head_dim=64, device="cpu", **kw)
+
+    def copy(src, dst, stream=None):
+        assert len(set(dst)) == len(dst) and not set(src) & set(dst)
+        c.k[:, dst], c.v[:, dst] = c.k[:, src], c.v[:, src]
+
+    c.copy_pages = copy  # the device copy, restated for CPU tensors
+    return c
+
+
+def fill(c, seq, first, values):
+    """Token first + i of the session holds the number values[i]."""
+    for i, x in enumerate(values):
+        page = c.pages_of(seq)[(first + i) // 16]
+        c.k[:, page, :, (first + i) % 16] = x
+        c.v[:, page, :, (first + i) % 16] = -x
+
+
+def read(c, seq, first=0):
+    out = []
+    for i in range(first, c.length(seq)):
+        page = c.pages_of(seq)[i // 16]
+        out.append(float(c.k[0, page, 0, i % 16, 0]))
+        assert float(c.v[1, page, 1, i % 16, 63]) == -out[-1]
+    return out
+
+
+def owned(c):
+    """Every page is free or referenced as often as the sessions list it."""
+    held = [p for s in c.sessions for p in c.pages_of(s) if p >= 0]
+    for p in range(c.pages):
+        assert c._refs[p] == held.count(p)
+    assert sorted(c._free) == [p for p in range(c.pages) if p not in held]
+
+
+def test_step_plan_arrays(pkg):
+    c = make(pkg)
+    a, b = c.new(), c.new()
+    s = c.step([a, b], [20, 3])
+    assert s.cu_q.tolist() == [0, 20, 23] and s.kv_len.tolist() == [20, 3]
+    assert s.page_table.tolist() == [c.pages_of(a), c.pages_of(b) + [-1]]
+    pa, pb = c.pages_of(a), c.pages_of(b)
+    assert s.slots.tolist() == ([pa[0] * 16 + i for i in range(16)] + [pa[1] * 16 + i for i in range(4)]
+                                + [pb[0] * 16 + i for i in range(3)])
+    assert (s.max_q, s.max_kv) == (20, 32)
+    again = c.step([b, a], [1, 0], extend=False)  # the last token of b anew, a only looked at
+    assert again.slots.tolist() == [pb[0] * 16 + 2] and again.kv_len.tolist() == [3, 20]
+    assert not s.stale and c.length(b) == 3
+    owned(c)
+
+
+def test_fork_shares_until_written(pkg):
+    c = make(pkg)
+    a = c.new()
+    c.step([a], 20)
+    fill(c, a, 0, range(20))
+    b, d = c.fork(a, 2)
+    assert c.free_pages == 10 and c.pages_of(b) == c.pages_of(a)
+    c.step([a, b, d], [1, 2, 0])  # a and b write into the shared second page, d keeps it
+    owned(c)
+    assert len({c.pages_of(x)[1] for x in (a, b, d)}) == 3
+    assert len({c.pages_of(x)[0] for x in (a, b, d)}) == 1
+    fill(c, a, 20, [100])
+    fill(c, b, 20, [200, 201])
+    base = [float(i) for i in range(20)]
+    assert read(c, a) == base + [100] and read(c, b) == base + [200, 201] and read(c, d) == base
+    c.step([d], 1)  # the last sharer writes in place
+    assert c.free_pages == 12 - 4
+    c.step([b], 20, extend=False)  # rewriting back into the shared first page copies it
+    assert c.pages_of(b)[0] != c.pages_of(a)[0] and read(c, b)[:2] == [0.0, 1.0]
+    owned(c)
+    for s in (a, b, d):
+        c.free(s)
+    assert c.free_pages == 12
+
+
+def test_full_cache_refuses_and_changes_nothing(pkg):
+    c = make(pkg, pages=3)
+    a = c.new()
+    c.step([a], 40)
+    b = c.fork(a)[0]
+    before = (c.pages_of(a), c.pages_of(b), list(c._refs), list(c._free))
+    with pytest.raises(RuntimeError, match="1 pages needed, 0 free"):
+        c.step([a, b], 1)
+    assert before == (c.pages_of(a), c.pages_of(b), list(c._refs), list(c._free)) and c.length(a) == 40
+
+
+def test_evict_truncate_compact(pkg):
+    c = make(pkg, pages=20)
+    a, b = c.new(), c.new()
+    c.step([a, b], [100, 40])
+    fill(c, a, 0, range(100))
+    fill(c, b, 0, range(200, 240))
+    # the next token (100) sees 70..100 and 0..3: pages of 16..63 go
+    assert c.evict(a, window=31, sinks=4) == 3
+    assert [p < 0 for p in c.pages_of(a)] == [False, True, True, True, False, False, False]
+    assert c.evict(a, window=31, sinks=4) == 0
+    owned(c)
+    c.truncate(b, 17)
+    assert c.free_pages == 20 - 4 - 2
+    old = c.step([b], 0)
+    assert c.compact() == 6 and old.stale
+    assert sorted(p for s in (a, b) for p in c.pages_of(s) if p >= 0) == list(range(6))
+    owned(c)
+    assert read(c, b) == [float(x) for x in range(200, 217)]
+    assert read(c, a, 64) == [float(x) for x in range(64, 100)]
+    with pytest.raises(ValueError, match="evicted page"):
+        c.step([a], 60, extend=False)
+    # frames of 10 tokens, window of 2 frames: token 100 (frame 10) sees from token 90 on
+    assert c.evict(a, window=2, frame_tokens=10) == 2 and c.pages_of(a)[:5] == [-1] * 5
+
+
+def test_plans_go_stale_and_are_rebuilt(pkg):
+    c = make(pkg)
+    a, b = c.new(), c.new()
+    s = c.step([a, b], 1, table_width=4)
+    assert s.max_kv == 64
+    buf = s.kv_len.data_ptr()
+    c.step([a, b], 1, into=s)
+    assert s.kv_len.tolist() == [2, 2] and s.kv_len.data_ptr() == buf and not s.stale
+    c.step([a], 1)
+    with pytest.raises(ValueError, match="out of date"):
+        c.attend(0, s, torch.zeros(2, 2, 64))
+    with pytest.raises(ValueError, match="room for 4"):
+        c.step([a, b], [80, 1], into=s)
+    with pytest.raises(ValueError, match="2 sessions and 2 tokens"):
+        c.step([a, b], [2, 1], into=s)
+    other = c.new()
+    c.step([a, other], 1, into=s)
+    c.free(b)  # no longer one of the plan's
+    assert not s.stale
+    c.free(other)
+    assert s.stale
+
+
+@pytest.mark.parametrize("bad", ["twice", "none", "unknown", "negative", "few", "rewrite"])
+def test_step_refusals(pkg, bad):
+    c = make(pkg)
+    a, b = c.new(), c.new()
+    args = {"twice": ([a, a], 1), "none": ([], 1), "unknown": ([a, 9], 1), "negative": ([a], -1),
+            "few": ([a, b], [1]), "rewrite": ([a], 1)}[bad]
+    with pytest.raises(ValueError):
+        c.step(*args, extend=bad != "rewrite")
+    assert c.free_pages == 12 and c.length(a) == 0
+
+
+def test_cache_refusals(pkg):
+    for kw in (dict(page_tokens=8), dict(head_dim=80), dict(dtype=torch.float32), dict(pages=0)):
+        args = dict(layers=1, pages=2, device="cpu")
+        args.update(kw)
+        with pytest.raises(ValueError):
+            pkg.PagedKVCacheB200(**args)
+    c = make(pkg)
+    a = c.new()
+    for call in (lambda: c.fork(a, -1), lambda: c.truncate(a, 1), lambda: c.evict(a, 0), lambda: c.free(7),
+                 lambda: c.adopt(c, a)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_axis_frequencies(pkg):
+    f = pkg.rope_axis_freqs((4, 2, 6), theta=(100.0, 7.0, 10000.0), device="cpu")
+    want = [1.0, 0.1, 1.0] + [10000.0 ** (-2 * i / 6) for i in range(3)]
+    assert f.dtype == torch.float64
+    np.testing.assert_allclose(f.numpy(), want, rtol=1e-15)
+    for axes, theta in (((3,), 10.0), ((), 10.0), ((4,), -1.0), ((4, 4), (1.0,))):
+        with pytest.raises(ValueError):
+            pkg.rope_axis_freqs(axes, theta, device="cpu")
+
+
+# ---------------------------------------------------------------- refusals of the C entry points
+
+
+def pages(pkg, **kw):
+    f = dict(k=16, v=1 << 40, layers=1, pages=4, kv_heads=2, page_tokens=16, head_dim=64, dtype=0)
+    f.update(kw)
+    return pkg._native.Pages(**f)
+
+
+def copy(pkg, src, dst, a, b):
+    i32 = ctypes.c_int32 * max(1, len(a))
+    return pkg.lib().oasis_pages_copy(src, dst, i32(*a), i32(*b), len(a), None)
+
+
+@pytest.mark.parametrize("change,a,b,status", [
+    ({}, [0, 1], [2, 2], 1),                # a destination twice
+    ({}, [0, 1], [1, 2], 1),                # source and destination at once
+    ({}, [0], [4], 1), ({}, [-1], [2], 1), ({}, [4], [2], 1),
+    ({"pages": 5}, [0], [1], 1),            # the same pool, another size
+    ({"k": 32}, [0], [1], 1),               # overlapping pools
+    ({"kv_heads": 1}, [0], [1], 1), ({"dtype": 1}, [0], [1], 1), ({"dtype": 2}, [0], [1], 6),
+    ({"v": (1 << 40) + 8}, [0], [1], 2), ({"k": None}, [0], [1], 1), ({"pages": 0}, [0], [1], 1),
+    ({"pages": 1 << 28}, [0], [1], 6),
+])
+def test_pages_copy_refusals(pkg, change, a, b, status):
+    assert copy(pkg, pages(pkg), pages(pkg, **change), a, b) == status
+    assert b"oasis_pages_copy" in pkg.lib().oasis_last_error()
+
+
+def test_pages_copy_of_nothing(pkg):
+    assert copy(pkg, pages(pkg), pages(pkg), [], []) == 0
+
+
+def rope_args(pkg, **kw):
+    f = dict(q=16, k=16, v=None, q_out=16, k_out=16, q_token_stride=128, q_head_stride=64, k_token_stride=128,
+             k_head_stride=64, v_token_stride=128, v_head_stride=64, q_out_token_stride=128,
+             q_out_head_stride=64, k_out_token_stride=128, k_out_head_stride=64, tokens=4, heads=2,
+             kv_heads=2, head_dim=64, dtype=0, norm=1, interleaved=1, eps=1e-6, q_weight=None, k_weight=None,
+             positions=16, positions_64=0, freqs=16, axes=3, axis_dims=(16, 24, 24), slots=None)
+    f.update(kw)
+    return pkg._native.QkNormRope(**f)
+
+
+@pytest.mark.parametrize("change,status", [
+    ({"tokens": -1}, 1), ({"heads": 0}, 1), ({"dtype": 3}, 6), ({"head_dim": 80}, 6), ({"axes": 0}, 1),
+    ({"axes": 5}, 1), ({"axis_dims": (16, 24, 25)}, 1), ({"axis_dims": (16, 24, 26)}, 1),
+    ({"axis_dims": (16, 24, 0)}, 1), ({"interleaved": 0, "axis_dims": (16, 24, 16)}, 6),
+    ({"norm": 0, "q_weight": 16}, 1), ({"q": None}, 1), ({"k_out": None}, 1), ({"positions": None}, 1),
+    ({"freqs": None}, 1), ({"q": 24}, 2), ({"q_head_stride": 63}, 2), ({"k_out_token_stride": 4}, 2),
+])
+def test_qk_norm_rope_refusals(pkg, change, status):
+    assert pkg.lib().oasis_qk_norm_rope(rope_args(pkg, **change), None) == status
+    assert b"oasis_qk_norm_rope" in pkg.lib().oasis_last_error()
+
+
+@pytest.mark.parametrize("page,change,status", [
+    ({}, {"v": None}, 1), ({}, {"slots": None}, 1), ({"layers": 2}, {}, 1), ({"kv_heads": 1}, {}, 1),
+    ({"head_dim": 128}, {}, 1), ({"dtype": 1}, {}, 1), ({"k": 8}, {}, 2), ({}, {"v": 24}, 2),
+])
+def test_qk_norm_rope_append_refusals(pkg, page, change, status):
+    args = dict(v=16, k_out=None, slots=16)
+    args.update(change)
+    args["pages"] = ctypes.pointer(pages(pkg, **page))
+    assert pkg.lib().oasis_qk_norm_rope(rope_args(pkg, **args), None) == status
+
+
+def test_no_tokens_launch_nothing(pkg):
+    assert pkg.lib().oasis_qk_norm_rope(rope_args(pkg, tokens=0), None) == 0
+    assert pkg.lib().oasis_attn_window(attn_args(pkg, tokens=0, batch=0), None) == 0
+
+
+def attn_args(pkg, **kw):
+    f = dict(q=16, out=16, lse=None, q_token_stride=128, q_head_stride=64, out_token_stride=128, out_head_stride=64,
+             k=16, v=1 << 40, pages=4, kv_heads=2, page_tokens=16, head_dim=64, dtype=0, page_table=16,
+             table_width=2, kv_len=16, cu_q=16, batch=1, tokens=4, heads=2, max_q=0, max_kv=0, window=0,
+             sinks=0, frame_tokens=1, scale=0.125)
+    f.update(kw)
+    return pkg._native.AttnWindow(**f)
+
+
+@pytest.mark.parametrize("change,status", [
+    ({"heads": 3}, 1), ({"heads": 0}, 1), ({"batch": -1}, 1), ({"table_width": 0}, 1), ({"window": -1}, 1),
+    ({"sinks": -1}, 1), ({"frame_tokens": 0}, 1), ({"head_dim": 96}, 6), ({"page_tokens": 24}, 6),
+    ({"dtype": 2}, 6), ({"scale": 0.0}, 1), ({"scale": float("nan")}, 1), ({"scale": float("inf")}, 1),
+    ({"batch": 65536}, 6), ({"table_width": 1 << 27}, 6), ({"cu_q": None}, 1), ({"q": None}, 1),
+    ({"kv_len": None}, 1), ({"k": None}, 1), ({"v": 24}, 2), ({"out": 24}, 2), ({"q_head_stride": 68}, 2),
+    ({"pages": 0}, 1), ({"pages": 1 << 28}, 6),
+])
+def test_attn_window_refusals(pkg, change, status):
+    assert pkg.lib().oasis_attn_window(attn_args(pkg, **change), None) == status
+    assert b"oasis_attn_window" in pkg.lib().oasis_last_error()
+
+
+def test_paged_struct_layouts_match_header(pkg):
+    """The ctypes mirrors have the C layouts."""
+    n = pkg._native
+    assert ctypes.sizeof(n.Pages) == 40
+    assert (n.QkNormRope.tokens.offset, n.QkNormRope.q_weight.offset, n.QkNormRope.axis_dims.offset,
+            n.QkNormRope.pages.offset, ctypes.sizeof(n.QkNormRope)) == (120, 152, 196, 216, 232)
+    assert (n.AttnWindow.k.offset, n.AttnWindow.page_table.offset, n.AttnWindow.cu_q.offset,
+            n.AttnWindow.scale.offset, ctypes.sizeof(n.AttnWindow)) == (56, 96, 120, 160, 168)
