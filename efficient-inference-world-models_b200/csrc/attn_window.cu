@@ -3,6 +3,10 @@
 //   out = softmax(scale q K^T over the visible keys) V,  key j visible to position p iff
 //   j < kv_len, j / F <= p / F and (W == 0 or p / F - j / F < W or j / F < S).
 // The visible keys of a position are two runs: [0, sink_end) and [start, end).
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
 #include "launch.cuh"
 
 namespace oasis {
@@ -71,7 +75,7 @@ __device__ __forceinline__ __half from_float(float x) { return __float2half_rn(x
 // One query row by one warp, key after key with the running maximum and sum: each lane holds
 // D / 32 dims.  Reads only what the row sees.
 template <typename T, int D>
-__device__ void window_row(const WinArgs& a, int b, const WinSeq& s, int qi, int head, int lane) {
+__device__ __noinline__ void window_row(const WinArgs& a, int b, const WinSeq& s, int qi, int head, int lane) {
   constexpr int E = D / 32;
   const long long row = s.q0 + qi;
   const T* q = static_cast<const T*>(a.q) + row * a.q_ts + head * a.q_hs + lane * E;
@@ -128,8 +132,57 @@ __global__ void __launch_bounds__(128) attn_window_rows_kernel(const __grid_cons
     window_row<T, D>(a, b, s, qi, blockIdx.y, lane);
 }
 
+}  // namespace oasis
+
+#include "attn_window_tile.cuh"
+
+namespace oasis {
+
+// Dynamic shared memory of a kernel above 48 KB, set once per device.
+template <auto Kernel>
+int allow_smem(int bytes, const char* what) {
+  static std::atomic<uint64_t> done{0};  // one per kernel
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e, what);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && (done.load(std::memory_order_acquire) & bit)) return OASIS_OK;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return cuda_status(e, what);
+  done.fetch_or(bit, std::memory_order_release);
+  return OASIS_OK;
+}
+
+// Rows of one page that a box of at most `most` rows can always take whole.
+inline int page_box(int page_tokens, int most) {
+  int r = 16;
+  while (r < most && page_tokens % (2 * r) == 0) r *= 2;
+  return r;
+}
+
+// The pages of one tensor as rows of D elements; boxes of 64 elements x box_rows.
+int encode_page_rows(CUtensorMap* map, const void* base, const WinArgs& a, int d, int box_rows) {
+  const long long dims[2] = {d, static_cast<long long>(a.pages) * a.kv_heads * a.page_tokens};
+  const long long strides[1] = {static_cast<long long>(d) * 2};
+  const int box[2] = {64, box_rows};
+  return encode_bf16_sw128(map, base, 2, dims, strides, box);
+}
+
 template <typename T, int D>
 int launch_attn_window(const WinArgs& a, int max_q, int max_kv, cudaStream_t stream) {
+  const long long max_rows = static_cast<long long>(max_q) * a.group;
+  if (max_rows > 16) {
+    const int box = page_box(a.page_tokens, kWtKeys);
+    CUtensorMap tk, tv;
+    if (int st = encode_page_rows(&tk, a.k, a, D, box)) return st;
+    if (int st = encode_page_rows(&tv, a.v, a, D, box)) return st;
+    if (int st = allow_smem<attn_window_tile_kernel<T, D>>(WtShape<D>::kSmem, "attn_window_tile_kernel")) return st;
+    const int row_tiles = static_cast<int>((max_rows + 2 * kWtRows - 1) / (2 * kWtRows));
+    cudaError_t e = launch_pdl(attn_window_tile_kernel<T, D>, dim3(row_tiles * a.kv_heads, 1, a.batch),
+                               dim3(kWtThreads), WtShape<D>::kSmem, stream, a, tk, tv, box, row_tiles);
+    if (e != cudaSuccess) return cuda_status(e, "attn_window_tile_kernel");
+    return OASIS_OK;
+  }
   cudaError_t e = launch_pdl(attn_window_rows_kernel<T, D>, dim3((max_q + 3) / 4, a.heads, a.batch), dim3(128), 0,
                              stream, a);
   if (e != cudaSuccess) return cuda_status(e, "attn_window_rows_kernel");

@@ -1,0 +1,532 @@
+// Window attention for prompts and frames: 256 query rows of one (sequence, key head) per CTA
+// on tcgen05, keys and values by TMA.  Included by attn_window.cu.
+//
+// Rows are the queries of the key head's group, token-major (row r: token r / group, head
+// r % group), so grouped heads share every key tile.  A CTA holds two tiles of 128 rows.
+// Roles: warps 0-3 and 4-7 are the softmax of tile 0 and 1 (one row per thread, S read from
+// TMEM); warp 8 issues the MMAs; warp 9 loads K and V tiles of 128 keys page by page; warps
+// 10-11 look over the V tiles that some row sees only in part.
+//
+// For tile i and key tile j:  S_i = Q_i K_j^T (TMEM, 128 columns), the softmax thread takes
+// P = exp2(S * scale - m) and writes it in 16 bits over S, O_i += P_i V_j (P from TMEM).  The MMA warp
+// alternates PV_0(j), QK_0(j+1), PV_1(j), QK_1(j+1): while one tile's softmax runs, the tensor
+// cores work for the other.  m is the running maximum, moved (and O rescaled) only when it
+// grows by more than 2^8, which keeps every p below 2^8 and the sum exact to fp32.
+#pragma once
+
+namespace oasis {
+
+constexpr int kWtRows = 128;     // query rows of a tile
+constexpr int kWtKeys = 128;     // keys of a K/V tile
+constexpr int kWtThreads = 384;  // 8 softmax warps, MMA, TMA, 2 V warps
+constexpr float kWtLazy = 8.0f;  // log2 of how far scores may pass the maximum in use
+
+template <int D>
+struct WtShape {
+  static constexpr int kHalf = kWtKeys * 128;              // 16 KB: 128 rows of 64 elements
+  static constexpr int kTile = kHalf * (D / 64);           // one Q, K or V tile
+  // even: K tiles take the even slots, V tiles the odd ones, so a barrier's phases are all of one kind
+  static constexpr int kStages = D == 128 ? 4 : 8;
+  static constexpr int kBars = 3 * kStages + 8;
+  static constexpr int kSmem = (2 + kStages) * kTile + 1024 + 256 + 8 * kBars;
+};
+
+// V tile as an MN-major operand: blocks of 64 dims (one swizzle atom) kHalf bytes apart.
+__device__ __forceinline__ uint64_t wt_v_desc(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>((kWtKeys * 128) >> 4) << 16;  // leading byte offset: next 64 dims
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;            // stride byte offset: next 8 keys
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;  // SWIZZLE_128B
+  return d;
+}
+
+// The block starts with 384 threads x 168 registers; the softmax warpgroups take what the
+// others give up: 256 x 208 + 128 x 88 = 384 x 168.
+template <int N>
+__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// P (A operand, K-major) from TMEM, V (B operand) from shared memory.
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      : "memory");
+}
+
+// 32 columns of this warp's 32 lanes, not waited for.
+__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Whether one of the two 16-bit values of a word is an infinity or NaN.
+template <typename T>
+__device__ __forceinline__ bool nonfinite2(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  return (w & e) == e || (w & (e << 16)) == (e << 16);
+}
+
+// Instruction descriptor of kind::f16 for this type: fp32 D, A K-major, B K-major or (b_mn) MN-major.
+template <typename T>
+__host__ __device__ constexpr uint32_t umma_idesc(int m, int n, bool b_mn) {
+  return (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10)) | (b_mn ? (1u << 16) : 0u) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// What a run of rows of one CTA sees, from the ranges of its first and last row (both ends of a
+// row's range only grow from row to row).
+struct WtSpan {
+  WinRange lo, hi;
+  bool any;
+  __device__ __forceinline__ bool all(int k0, int k1) const {  // every row sees all of [k0, k1)
+    return k1 <= lo.end && (k0 >= hi.start || k1 <= lo.sink_end);
+  }
+  __device__ __forceinline__ bool some(int k0, int k1) const {  // some row may see some of it
+    return any && k0 < hi.end && (k1 > lo.start || k0 < hi.sink_end);
+  }
+  __device__ __forceinline__ bool sees(int key) const {
+    return key < hi.end && (key >= lo.start || key < hi.sink_end);
+  }
+};
+__device__ __forceinline__ WtSpan wt_span(const WinArgs& a, const WinSeq& s, int row0, int row1) {
+  WtSpan w;
+  const int base = s.kv - s.n_q;
+  const int p1 = base + (row1 - 1) / a.group;
+  w.any = row0 < row1 && p1 >= 0;
+  w.lo = win_range(a, base + row0 / a.group, s.kv);  // all zero where the position is negative
+  w.hi = win_range(a, p1, s.kv);
+  return w;
+}
+
+// The key tiles of a span: [0, sink) and [first, last).
+struct WtTiles {
+  int sink, first, n;
+  __device__ __forceinline__ int tile(int j) const { return j < sink ? j : first + j - sink; }
+};
+__device__ __forceinline__ WtTiles wt_tiles(const WtSpan& w, int keys) {
+  WtTiles t = {0, 0, 0};
+  if (!w.any) return t;
+  t.sink = (min(w.hi.sink_end, w.lo.start) + keys - 1) / keys;
+  t.first = max(w.lo.start / keys, t.sink);
+  t.n = t.sink + max(0, (w.hi.end + keys - 1) / keys - t.first);
+  return t;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kWtThreads, 1)
+    attn_window_tile_kernel(const __grid_constant__ WinArgs a, const __grid_constant__ CUtensorMap tm_k,
+                            const __grid_constant__ CUtensorMap tm_v, int box_rows, int row_tiles) {
+  using S = WtShape<D>;
+  constexpr int kStages = S::kStages;
+  extern __shared__ uint8_t wt_raw[];
+  uint8_t* sQ = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(wt_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* ring = sQ + 2 * S::kTile;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * S::kTile);
+  uint64_t* clean = full + kStages;
+  uint64_t* empty = clean + kStages;
+  uint64_t* q_full = empty + kStages;
+  uint64_t* s_full = q_full + 1;   // [2]
+  uint64_t* p_full = s_full + 2;   // [2]
+  uint64_t* pv_done = p_full + 2;  // [2]
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(pv_done + 3);
+  uint32_t* dirty = tmem_holder + 1;
+
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&clean[i], 2);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(q_full, 8);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    *dirty = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 8) tmem_alloc<512>(tmem_holder);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  pdl_wait();
+
+  const int b = blockIdx.z;
+  const WinSeq seq = win_seq(a, b);
+  const int rows = seq.n_q * a.group;
+  // later rows of a causal prompt see more: they start first
+  const int tile_id = row_tiles - 1 - static_cast<int>(blockIdx.x) / a.kv_heads;
+  const int kvh = static_cast<int>(blockIdx.x) % a.kv_heads;
+  const int row0 = tile_id * (2 * kWtRows);
+  const int32_t* table = a.table + static_cast<long long>(b) * a.width;
+  const int row1 = min(rows, row0 + 2 * kWtRows);
+  const WtSpan span = wt_span(a, seq, row0, row1);
+  const WtSpan half[2] = {wt_span(a, seq, row0, min(row1, row0 + kWtRows)),
+                          wt_span(a, seq, min(row1, row0 + kWtRows), row1)};
+  const WtTiles tiles = wt_tiles(span, kWtKeys);
+  const int n = tiles.n;
+
+  if (warp >= 8) {
+    reg_dec<88>();
+    if (row0 >= rows) {
+      // nothing to do
+    } else if (warp == 9) {
+      if (lane == 0) {
+        // ------------------------------------------------------------ TMA: K0 V0 K1 V1 ...
+        const int boxes = kWtKeys / box_rows, page_boxes = a.page_tokens / box_rows;
+        const int none = a.pages * a.kv_heads * a.page_tokens;  // beyond the pages: zeros
+        bool ok = true;
+        int it = 0;
+        for (int j = 0; j < n && ok; ++j) {
+          const int box0 = tiles.tile(j) * boxes;
+          for (int kv = 0; kv < 2 && ok; ++kv, ++it) {
+            const int st = it % kStages;
+            if (it >= kStages) ok = mbar_wait(&empty[st], ((it / kStages) - 1) & 1);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&full[st], S::kTile);
+            uint8_t* dst = ring + st * S::kTile;
+            for (int x = 0; x < boxes; ++x) {
+              const int idx = (box0 + x) / page_boxes;
+              const int page = idx < a.width ? table[idx] : -1;
+              const int row = page >= 0 && page < a.pages
+                                  ? (page * a.kv_heads + kvh) * a.page_tokens + ((box0 + x) % page_boxes) * box_rows
+                                  : none;
+#pragma unroll
+              for (int h = 0; h < D / 64; ++h) {
+                uint8_t* to = dst + h * S::kHalf + x * box_rows * 128;
+                // (two calls: a selected pointer would make the compiler copy the maps to the stack)
+                if (kv)
+                  tma_load_2d(to, &tm_v, &full[st], h * 64, row);
+                else
+                  tma_load_2d(to, &tm_k, &full[st], h * 64, row);
+              }
+            }
+          }
+        }
+        if (!ok)  // gave up: let the copies in flight land before the memory is given back
+          for (int i = max(0, it - kStages); i < it; ++i) mbar_wait(&full[i % kStages], (i / kStages) & 1);
+      }
+    } else if (warp == 8) {
+      if (lane == 0) {
+        // ------------------------------------------------------------ MMA
+        constexpr uint32_t idesc_s = umma_idesc<T>(kWtRows, kWtKeys, false);
+        constexpr uint32_t idesc_o = umma_idesc<T>(kWtRows, D, true);
+        const uint32_t q_addr = smem_u32(sQ), ring_addr = smem_u32(ring);
+        auto qk = [&](int i, int st) {
+          const uint32_t qa = q_addr + i * S::kTile, ka = ring_addr + st * S::kTile;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_bf16(tmem + i * 128, umma_desc_sw128(qa + (k >> 2) * S::kHalf + (k & 3) * 32),
+                      umma_desc_sw128(ka + (k >> 2) * S::kHalf + (k & 3) * 32), idesc_s, k > 0);
+          umma_commit(&s_full[i]);
+        };
+        auto pv = [&](int i, int st, bool acc) {
+          const uint32_t va = ring_addr + st * S::kTile;
+#pragma unroll
+          for (int k = 0; k < kWtKeys / 16; ++k)
+            umma_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8,
+                    wt_v_desc(va + k * 2048), idesc_o, acc || k > 0);
+          umma_commit(&pv_done[i]);
+        };
+        bool ok = mbar_wait(q_full, 0);
+        uint32_t np[2] = {0, 0};  // P tiles taken
+        if (ok && n > 0) {
+          const int t0 = tiles.tile(0) * kWtKeys;
+          ok = mbar_wait(&full[0], 0);
+          if (ok) {
+            tc_fence_after();
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (half[i].some(t0, t0 + kWtKeys)) qk(i, 0);
+            umma_commit(&empty[0]);
+          }
+        }
+        for (int j = 0; j < n && ok; ++j) {
+          const int k0 = tiles.tile(j) * kWtKeys, k1 = j + 1 < n ? tiles.tile(j + 1) * kWtKeys : 0;
+          const int vi = 2 * j + 1, ki = 2 * j + 2;
+          const int vs = vi % kStages, ks = ki % kStages;
+          ok = mbar_wait(&clean[vs], (vi / kStages) & 1);
+          if (ok && j + 1 < n) ok = mbar_wait(&full[ks], (ki / kStages) & 1);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (half[i].some(k0, k0 + kWtKeys)) {
+              ok = ok && mbar_wait(&p_full[i], np[i] & 1);
+              if (!ok) break;
+              tc_fence_after();
+              pv(i, vs, np[i] > 0);
+              ++np[i];
+            }
+            if (j + 1 < n && half[i].some(k1, k1 + kWtKeys)) qk(i, ks);
+          }
+          if (!ok) break;
+          umma_commit(&empty[vs]);
+          if (j + 1 < n) umma_commit(&empty[ks]);
+        }
+      }
+    } else {
+      // -------------------------------------------------------------- V tiles seen in part
+      // Zeroes the rows that no query of this CTA sees (ends of pages, tokens before the window):
+      // their weights are 0, but 0 * NaN is not.  An infinity or NaN in a row that only some of
+      // the queries see marks the CTA: its rows are then computed one by one (window_row).
+      const int w = warp - 10;
+      bool ok = true;
+      for (int j = 0; j < n && ok; ++j) {
+        const int vi = 2 * j + 1, st = vi % kStages;
+        const int k0 = tiles.tile(j) * kWtKeys;
+        ok = mbar_wait(&full[st], (vi / kStages) & 1);
+        if (ok && !span.all(k0, k0 + kWtKeys)) {
+          uint8_t* v = ring + st * S::kTile;
+          bool bad = false;
+          for (int r = w * (kWtKeys / 2) + lane / 8; r < (w + 1) * (kWtKeys / 2); r += 4) {
+            const bool seen = span.sees(k0 + r);
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) {
+              uint4* p = reinterpret_cast<uint4*>(v + h * S::kHalf + r * 128 + (lane % 8) * 16);
+              if (seen) {
+                const uint4 x = *p;
+                bad |= nonfinite2<T>(x.x) || nonfinite2<T>(x.y) || nonfinite2<T>(x.z) || nonfinite2<T>(x.w);
+              } else {
+                *p = make_uint4(0, 0, 0, 0);
+              }
+            }
+          }
+          if (bad) *dirty = 1;
+          fence_async_smem_cta();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&clean[st]);
+      }
+    }
+  } else {
+    reg_inc<208>();
+    if (row0 < rows) {
+      // -------------------------------------------------------------- softmax
+      const int i = warp >> 2;                  // tile
+      const int quarter = warp & 3;             // TMEM lanes of this warp
+      const int r = quarter * 32 + lane;        // row in the tile
+      const int row = row0 + i * kWtRows + r;   // row of the (sequence, key head)
+      // Q rows of this warp into the swizzled tile, zeros past the end
+      uint8_t* q_tile = sQ + i * S::kTile;
+      constexpr int kChunks = D / 8;
+#pragma unroll
+      for (int x = 0; x < kChunks; ++x) {
+        const int c = x * 32 + lane;
+        const int rr = quarter * 32 + c / kChunks, ch = c % kChunks;
+        const int qrow = row0 + i * kWtRows + rr;
+        uint4 val = make_uint4(0, 0, 0, 0);
+        if (qrow < row1) {
+          const T* src = static_cast<const T*>(a.q) + static_cast<long long>(seq.q0 + qrow / a.group) * a.q_ts +
+                         (kvh * a.group + qrow % a.group) * a.q_hs + ch * 8;
+          val = *reinterpret_cast<const uint4*>(src);
+        }
+        *reinterpret_cast<uint4*>(q_tile + (ch >> 3) * S::kHalf + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = val;
+      }
+      fence_async_smem_cta();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+
+      const WinRange range =
+          row < row1 ? win_range(a, seq.kv - seq.n_q + row / a.group, seq.kv) : WinRange{0, 0, 0};
+      const uint32_t s_addr = tmem + i * 128 + (static_cast<uint32_t>(quarter * 32) << 16);
+      const uint32_t o_addr = tmem + 256 + i * D + (static_cast<uint32_t>(quarter * 32) << 16);
+      const float sl2 = a.scale_log2;
+      const int boxes = kWtKeys / box_rows, page_boxes = a.page_tokens / box_rows;
+      float m = -INFINITY, l = 0.0f;
+      uint32_t np = 0;
+      bool ok = true;
+      for (int j = 0; j < n; ++j) {
+        const int tile = tiles.tile(j), k0 = tile * kWtKeys;
+        if (!half[i].some(k0, k0 + kWtKeys)) continue;
+        // pages that are not there (before the wait: the look-up runs under it)
+        bool hole = false;
+        if (lane < boxes) {
+          const int idx = (tile * boxes + lane) / page_boxes;
+          const int page = idx < a.width ? table[idx] : -1;
+          hole = page < 0 || page >= a.pages;
+        }
+        const uint32_t holes = __ballot_sync(0xffffffffu, hole);
+        ok = mbar_wait(&s_full[i], np & 1);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc_fence_after();
+        uint32_t sv[kWtKeys];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32_nowait(s_addr + c * 32, sv + c * 32);
+        tmem_wait_ld();
+        float* s = reinterpret_cast<float*>(sv);
+        if (holes || !half[i].all(k0, k0 + kWtKeys)) {
+#pragma unroll
+          for (int x = 0; x < kWtKeys; ++x) {
+            const int key = k0 + x;
+            bool see = range.sees(key);
+            if (holes) see = see && !((holes >> (x / box_rows)) & 1u);
+            s[x] = see ? s[x] : -INFINITY;
+          }
+        }
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int x = 4; x < kWtKeys; x += 4) {
+          mx[0] = fmaxf(mx[0], s[x]);
+          mx[1] = fmaxf(mx[1], s[x + 1]);
+          mx[2] = fmaxf(mx[2], s[x + 2]);
+          mx[3] = fmaxf(mx[3], s[x + 3]);
+        }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        // -inf - -inf is NaN and compares false: nothing seen yet keeps m
+        const bool grow = (top - m) * sl2 > kWtLazy;
+        float alpha = 1.0f;
+        if (grow) {
+          alpha = ex2((m - top) * sl2);  // 0 at the first tile
+          m = top;
+          l *= alpha;
+        }
+        if (np > 0 && __any_sync(0xffffffffu, grow)) {
+          ok = mbar_wait(&pv_done[i], (np - 1) & 1);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32_nowait(o_addr + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+            tmem_st32(o_addr + c * 32, o);
+          }
+        }
+        const float base = m == -INFINITY ? 0.0f : m * sl2;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t pk[kWtKeys / 2];
+#pragma unroll
+        for (int x = 0; x < kWtKeys; x += 4) {
+          float e[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            e[y] = ex2(fmaf(s[x + y], sl2, -base));
+            sum[y] += e[y];
+          }
+          pk[x / 2] = pack2<T>(e[0], e[1]);
+          pk[x / 2 + 1] = pack2<T>(e[2], e[3]);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st32(s_addr, pk);
+        tmem_st32(s_addr + 32, pk + 32);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[i]);
+        ++np;
+      }
+      if (ok && np > 0) ok = mbar_wait(&pv_done[i], (np - 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      // the V warps' mark: every tile they looked at was multiplied before pv_done
+      if (ok && *reinterpret_cast<volatile uint32_t*>(dirty)) {
+        for (int x = 0; x < 32; ++x) {
+          const int rr = row0 + i * kWtRows + quarter * 32 + x;
+          if (rr < row1) window_row<T, D>(a, b, seq, rr / a.group, kvh * a.group + rr % a.group, lane);
+        }
+      } else if (ok) {
+        // O / l through the warp's own rows of the Q tile (its last reader is done), then out in
+        // whole rows
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          if (np > 0) {
+            tmem_ld32_nowait(o_addr + c * 32, o);
+            tmem_wait_ld();
+          }
+          const bool some = np > 0 && inv != 0.0f;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint32_t w4[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              w4[y] = some ? pack2<T>(__uint_as_float(o[8 * x + 2 * y]) * inv, __uint_as_float(o[8 * x + 2 * y + 1]) * inv)
+                           : 0u;
+            const int ch = c * 4 + x;
+            *reinterpret_cast<uint4*>(q_tile + (ch >> 3) * S::kHalf + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) =
+                make_uint4(w4[0], w4[1], w4[2], w4[3]);
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int x = 0; x < kChunks; ++x) {
+          const int c = x * 32 + lane;
+          const int rr = quarter * 32 + c / kChunks, ch = c % kChunks;
+          const int orow = row0 + i * kWtRows + rr;
+          if (orow < row1) {
+            T* dst = static_cast<T*>(a.out) + static_cast<long long>(seq.q0 + orow / a.group) * a.o_ts +
+                     (kvh * a.group + orow % a.group) * a.o_hs + ch * 8;
+            *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(
+                q_tile + (ch >> 3) * S::kHalf + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4));
+          }
+        }
+        if (a.lse && row < row1)
+          a.lse[static_cast<long long>(seq.q0 + row / a.group) * a.heads + kvh * a.group + row % a.group] =
+              l == 0.0f ? -INFINITY : (m * sl2 + log2f(l)) * 0.6931471805599453f;
+      }
+    }
+    // more rows than the launch was told of: one by one
+    if (tile_id == row_tiles - 1)
+      for (int r = row_tiles * (2 * kWtRows) + warp; r < rows; r += 8)
+        window_row<T, D>(a, b, seq, r / a.group, kvh * a.group + r % a.group, lane);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) tmem_dealloc<512>(tmem);
+}
+
+}  // namespace oasis
