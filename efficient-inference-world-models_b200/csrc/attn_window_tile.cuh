@@ -72,7 +72,18 @@ __device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t* r) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The registers pass through the wait, so that nothing reads them before it.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                 "+r"(r[29])
+               :
+               : "memory");
+  asm volatile("" : "+r"(r[30]), "+r"(r[31])::"memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
   asm volatile(
@@ -84,6 +95,53 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// Pairs of fp32 in one 64-bit register: two multiply-adds or sums per instruction.
+__device__ __forceinline__ uint64_t pair_f32(uint32_t lo, uint32_t hi) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "r"(lo), "r"(hi));
+  return p;
+}
+__device__ __forceinline__ uint64_t pair_f32(float lo, float hi) {
+  return pair_f32(__float_as_uint(lo), __float_as_uint(hi));
+}
+__device__ __forceinline__ float2 unpair_f32(uint64_t p) {
+  uint32_t lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(p));
+  return make_float2(__uint_as_float(lo), __uint_as_float(hi));
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// Bits lo..hi-1 of a word, both clamped to it.
+__device__ __forceinline__ uint32_t wt_bits(int lo, int hi) {
+  lo = max(0, min(lo, 32));
+  hi = max(0, min(hi, 32));
+  const uint32_t below_hi = hi == 32 ? ~0u : (1u << hi) - 1u, below_lo = lo == 32 ? ~0u : (1u << lo) - 1u;
+  return below_hi & ~below_lo;
+}
+__device__ __forceinline__ void wt_hide(uint32_t (&v)[32], uint32_t seen) {
+#pragma unroll
+  for (int x = 0; x < 32; ++x)
+    if (!((seen >> x) & 1u)) v[x] = 0xff800000u;  // -inf
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -353,6 +411,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
     if (row0 < rows) {
       // -------------------------------------------------------------- softmax
       const int i = warp >> 2;                  // tile
+      const WtSpan mine = i ? half[1] : half[0];
       const int quarter = warp & 3;             // TMEM lanes of this warp
       const int r = quarter * 32 + lane;        // row in the tile
       const int row = row0 + i * kWtRows + r;   // row of the (sequence, key head)
@@ -387,7 +446,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       bool ok = true;
       for (int j = 0; j < n; ++j) {
         const int tile = tiles.tile(j), k0 = tile * kWtKeys;
-        if (!half[i].some(k0, k0 + kWtKeys)) continue;
+        if (!mine.some(k0, k0 + kWtKeys)) continue;
         // pages that are not there (before the wait: the look-up runs under it)
         bool hole = false;
         if (lane < boxes) {
@@ -399,28 +458,42 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         ok = mbar_wait(&s_full[i], np & 1);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
-        uint32_t sv[kWtKeys];
+        // S twice through 32 columns at a time (maximum, then weights): half the registers of
+        // holding the row, and TMEM reads are cheap beside the exponentials
+        const bool part = holes || !mine.all(k0, k0 + kWtKeys);
+        uint32_t seen[4] = {~0u, ~0u, ~0u, ~0u};
+        if (part) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32_nowait(s_addr + c * 32, sv + c * 32);
-        tmem_wait_ld();
-        float* s = reinterpret_cast<float*>(sv);
-        if (holes || !half[i].all(k0, k0 + kWtKeys)) {
+          for (int c = 0; c < 4; ++c) {
+            const int k = k0 + c * 32;
+            seen[c] = wt_bits(range.start - k, range.end - k) | wt_bits(-k, range.sink_end - k);
+            if (holes) {
 #pragma unroll
-          for (int x = 0; x < kWtKeys; ++x) {
-            const int key = k0 + x;
-            bool see = range.sees(key);
-            if (holes) see = see && !((holes >> (x / box_rows)) & 1u);
-            s[x] = see ? s[x] : -INFINITY;
+              for (int x = 0; x < 32; x += 16)
+                if ((holes >> ((c * 32 + x) / box_rows)) & 1u) seen[c] &= ~(0xffffu << x);
+            }
           }
         }
-        float mx[4] = {s[0], s[1], s[2], s[3]};
+        uint32_t sa[32], sb[32];
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto maxima = [&](uint32_t(&v)[32], uint32_t bits) {
+          if (part) wt_hide(v, bits);
 #pragma unroll
-        for (int x = 4; x < kWtKeys; x += 4) {
-          mx[0] = fmaxf(mx[0], s[x]);
-          mx[1] = fmaxf(mx[1], s[x + 1]);
-          mx[2] = fmaxf(mx[2], s[x + 2]);
-          mx[3] = fmaxf(mx[3], s[x + 3]);
-        }
+          for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(v[x]));
+        };
+        tmem_ld32_nowait(s_addr, sa);
+        tmem_wait_ld(sa);
+        tmem_ld32_nowait(s_addr + 32, sb);
+        maxima(sa, seen[0]);
+        tmem_wait_ld(sb);
+        tmem_ld32_nowait(s_addr + 64, sa);
+        maxima(sb, seen[1]);
+        tmem_wait_ld(sa);
+        tmem_ld32_nowait(s_addr + 96, sb);
+        maxima(sa, seen[2]);
+        tmem_wait_ld(sb);
+        tmem_ld32_nowait(s_addr, sa);
+        maxima(sb, seen[3]);
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         // -inf - -inf is NaN and compares false: nothing seen yet keeps m
         const bool grow = (top - m) * sl2 > kWtLazy;
@@ -430,37 +503,50 @@ __global__ void __launch_bounds__(kWtThreads, 1)
           m = top;
           l *= alpha;
         }
+        tmem_wait_ld(sa);
         if (np > 0 && __any_sync(0xffffffffu, grow)) {
           ok = mbar_wait(&pv_done[i], (np - 1) & 1);
           if (!__all_sync(0xffffffffu, ok)) break;
           tc_fence_after();
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
             tmem_ld32_nowait(o_addr + c * 32, o);
-            tmem_wait_ld();
+            tmem_wait_ld(o);
 #pragma unroll
             for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
             tmem_st32(o_addr + c * 32, o);
           }
         }
-        const float base = m == -INFINITY ? 0.0f : m * sl2;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        uint32_t pk[kWtKeys / 2];
+        const float base = m == -INFINITY ? 0.0f : -m * sl2;
+        uint64_t sum[2] = {0, 0};
+        // the columns of P lie over columns of S that have been read
+        auto weights = [&](uint32_t(&v)[32], uint32_t bits, int c) {
+          if (part) wt_hide(v, bits);
+          uint32_t pk[16];
 #pragma unroll
-        for (int x = 0; x < kWtKeys; x += 4) {
-          float e[4];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            e[y] = ex2(fmaf(s[x + y], sl2, -base));
-            sum[y] += e[y];
+          for (int x = 0; x < 32; x += 2) {
+            const uint64_t t = fma_f32x2(pair_f32(v[x], v[x + 1]), pair_f32(sl2, sl2), pair_f32(base, base));
+            float2 e = unpair_f32(t);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            sum[(x >> 1) & 1] = add_f32x2(sum[(x >> 1) & 1], pair_f32(e.x, e.y));
+            pk[x / 2] = pack2<T>(e.x, e.y);
           }
-          pk[x / 2] = pack2<T>(e[0], e[1]);
-          pk[x / 2 + 1] = pack2<T>(e[2], e[3]);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_st32(s_addr, pk);
-        tmem_st32(s_addr + 32, pk + 32);
+          tmem_st16(s_addr + c * 16, pk);
+        };
+        tmem_ld32_nowait(s_addr + 32, sb);
+        weights(sa, seen[0], 0);
+        tmem_wait_ld(sb);
+        tmem_ld32_nowait(s_addr + 64, sa);
+        weights(sb, seen[1], 1);
+        tmem_wait_ld(sa);
+        tmem_ld32_nowait(s_addr + 96, sb);
+        weights(sa, seen[2], 2);
+        tmem_wait_ld(sb);
+        weights(sb, seen[3], 3);
+        const float2 s2 = unpair_f32(add_f32x2(sum[0], sum[1]));
+        l += s2.x + s2.y;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -480,14 +566,14 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         // O / l through the warp's own rows of the Q tile (its last reader is done), then out in
         // whole rows
         const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-#pragma unroll
+        const bool some = np > 0 && inv != 0.0f;
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
+          uint32_t o[32] = {};
           if (np > 0) {
             tmem_ld32_nowait(o_addr + c * 32, o);
-            tmem_wait_ld();
+            tmem_wait_ld(o);
           }
-          const bool some = np > 0 && inv != 0.0f;
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             uint32_t w4[4];
