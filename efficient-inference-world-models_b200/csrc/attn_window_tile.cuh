@@ -4,8 +4,8 @@
 // Rows are the queries of the key head's group, token-major (row r: token r / group, head
 // r % group), so grouped heads share every key tile.  A CTA holds two tiles of 128 rows.
 // Roles: warps 0-3 and 4-7 are the softmax of tile 0 and 1 (one row per thread, S read from
-// TMEM); warp 8 issues the MMAs; warp 9 loads K and V tiles of 128 keys page by page; warps
-// 10-11 look over the V tiles that some row sees only in part.
+// TMEM); warp 8 issues the MMAs; warp 9 loads K and V tiles of 128 keys page by page and looks
+// over the V tiles that some row sees only in part.
 //
 // For tile i and key tile j:  S_i = Q_i K_j^T (TMEM, 128 columns), the softmax thread takes
 // P = exp2(S * scale - m) and writes it in 16 bits over S, O_i += P_i V_j (P from TMEM).  The MMA warp
@@ -18,16 +18,18 @@ namespace oasis {
 
 constexpr int kWtRows = 128;     // query rows of a tile
 constexpr int kWtKeys = 128;     // keys of a K/V tile
-constexpr int kWtThreads = 384;  // 8 softmax warps, MMA, TMA, 2 V warps
+constexpr int kWtThreads = 320;  // 8 softmax warps, MMA, loads: 200 registers each
+constexpr int kWtPolyEvery = 3;  // of the weights' pairs, one in three is computed without the SFU
 constexpr float kWtLazy = 8.0f;  // log2 of how far scores may pass the maximum in use
 
 template <int D>
 struct WtShape {
   static constexpr int kHalf = kWtKeys * 128;              // 16 KB: 128 rows of 64 elements
   static constexpr int kTile = kHalf * (D / 64);           // one Q, K or V tile
-  // even: K tiles take the even slots, V tiles the odd ones, so a barrier's phases are all of one kind
-  static constexpr int kStages = D == 128 ? 4 : 8;
-  static constexpr int kBars = 3 * kStages + 8;
+  // a K tile is done with a step before the V tile of the same keys: fewer of them
+  static constexpr int kStagesK = D == 128 ? 2 : 4, kStagesV = D == 128 ? 3 : 4;
+  static constexpr int kStages = kStagesK + kStagesV;
+  static constexpr int kBars = 3 * kStages + 10;
   static constexpr int kSmem = (2 + kStages) * kTile + 1024 + 256 + 8 * kBars;
 };
 
@@ -41,13 +43,6 @@ __device__ __forceinline__ uint64_t wt_v_desc(uint32_t smem_addr) {
   d |= static_cast<uint64_t>(2u) << 61;  // SWIZZLE_128B
   return d;
 }
-
-// The block starts with 384 threads x 168 registers; the softmax warpgroups take what the
-// others give up: 256 x 208 + 128 x 88 = 384 x 168.
-template <int N>
-__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // P (A operand, K-major) from TMEM, V (B operand) from shared memory.
 __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
@@ -129,6 +124,34 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
+}
+
+// The larger of three; NaN if one is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x of two fp32 on the multiply-add pipes: x = n + f with n the nearest integer (read off the
+// low bits of x + 1.5 2^23), 2^f by the minimax polynomial of degree 5 on [-1/2, 1/2] (found by
+// Remez exchange; relative error 2^-22 with fp32 rounding), n added to the exponent.  x is
+// kept above -126; not for NaN or infinities.
+__device__ __forceinline__ float2 exp2_poly(uint64_t x2) {
+  float2 x = unpair_f32(x2);
+  x2 = pair_f32(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
+  const uint64_t magic = pair_f32(12582912.0f, 12582912.0f), unmagic = pair_f32(-12582912.0f, -12582912.0f);
+  const uint64_t r = add_f32x2(x2, magic);
+  const uint64_t f = fma_f32x2(add_f32x2(r, unmagic), pair_f32(-1.0f, -1.0f), x2);
+  uint64_t p = pair_f32(0.0013276472454890609f, 0.0013276472454890609f);
+  p = fma_f32x2(p, f, pair_f32(0.009675540961325169f, 0.009675540961325169f));
+  p = fma_f32x2(p, f, pair_f32(0.05550713092088699f, 0.05550713092088699f));
+  p = fma_f32x2(p, f, pair_f32(0.24022120237350464f, 0.24022120237350464f));
+  p = fma_f32x2(p, f, pair_f32(0.6931469440460205f, 0.6931469440460205f));
+  p = fma_f32x2(p, f, pair_f32(1.0000001192092896f, 1.0000001192092896f));
+  const float2 e = unpair_f32(p), n = unpair_f32(r);
+  return make_float2(__uint_as_float(__float_as_uint(e.x) + (__float_as_uint(n.x) << 23)),
+                     __uint_as_float(__float_as_uint(e.y) + (__float_as_uint(n.y) << 23)));
 }
 
 // Bits lo..hi-1 of a word, both clamped to it.
@@ -218,7 +241,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
     attn_window_tile_kernel(const __grid_constant__ WinArgs a, const __grid_constant__ CUtensorMap tm_k,
                             const __grid_constant__ CUtensorMap tm_v, int box_rows, int row_tiles) {
   using S = WtShape<D>;
-  constexpr int kStages = S::kStages;
+  constexpr int kStages = S::kStages, kSK = S::kStagesK, kSV = S::kStagesV;  // slots: K, then V
   extern __shared__ uint8_t wt_raw[];
   uint8_t* sQ = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(wt_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* ring = sQ + 2 * S::kTile;
@@ -228,8 +251,9 @@ __global__ void __launch_bounds__(kWtThreads, 1)
   uint64_t* q_full = empty + kStages;
   uint64_t* s_full = q_full + 1;   // [2]
   uint64_t* p_full = s_full + 2;   // [2]
-  uint64_t* pv_done = p_full + 2;  // [2]
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(pv_done + 3);
+  uint64_t* p_half = p_full + 2;   // [2]
+  uint64_t* pv_done = p_half + 2;  // [2]
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(pv_done + 2);
   uint32_t* dirty = tmem_holder + 1;
 
   pdl_trigger();
@@ -237,13 +261,14 @@ __global__ void __launch_bounds__(kWtThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&clean[i], 2);
+      mbar_init(&clean[i], 1);
       mbar_init(&empty[i], 1);
     }
     mbar_init(q_full, 8);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
+      mbar_init(&p_half[i], 4);
       mbar_init(&pv_done[i], 1);
     }
     *dirty = 0;
@@ -274,119 +299,43 @@ __global__ void __launch_bounds__(kWtThreads, 1)
   const int n = tiles.n;
 
   if (warp >= 8) {
-    reg_dec<88>();
     if (row0 >= rows) {
       // nothing to do
     } else if (warp == 9) {
-      if (lane == 0) {
-        // ------------------------------------------------------------ TMA: K0 V0 K1 V1 ...
-        const int boxes = kWtKeys / box_rows, page_boxes = a.page_tokens / box_rows;
-        const int none = a.pages * a.kv_heads * a.page_tokens;  // beyond the pages: zeros
-        bool ok = true;
-        int it = 0;
-        for (int j = 0; j < n && ok; ++j) {
-          const int box0 = tiles.tile(j) * boxes;
-          for (int kv = 0; kv < 2 && ok; ++kv, ++it) {
-            const int st = it % kStages;
-            if (it >= kStages) ok = mbar_wait(&empty[st], ((it / kStages) - 1) & 1);
-            if (!ok) break;
-            mbar_arrive_expect_tx(&full[st], S::kTile);
-            uint8_t* dst = ring + st * S::kTile;
-            for (int x = 0; x < boxes; ++x) {
-              const int idx = (box0 + x) / page_boxes;
-              const int page = idx < a.width ? table[idx] : -1;
-              const int row = page >= 0 && page < a.pages
-                                  ? (page * a.kv_heads + kvh) * a.page_tokens + ((box0 + x) % page_boxes) * box_rows
-                                  : none;
+      // -------------------------------------------------------------- loads, and V tiles seen in part
+      // A V tile that some query does not see whole is looked over before the MMAs may have it:
+      // rows that no query of this CTA sees (ends of pages, tokens before the window) are zeroed, since
+      // their weights are 0 but 0 * NaN is not; an infinity or NaN in a row that only some queries
+      // see marks the CTA, whose rows are then computed one by one (window_row).
+      const int boxes = kWtKeys / box_rows, page_boxes = a.page_tokens / box_rows;
+      const int none = a.pages * a.kv_heads * a.page_tokens;  // beyond the pages: zeros
+      auto box_row = [&](int j) {  // lane x takes box x
+        const int box = tiles.tile(j) * boxes + lane;
+        const int idx = box / page_boxes;
+        const int page = idx < a.width ? table[idx] : -1;
+        return page >= 0 && page < a.pages
+                   ? (page * a.kv_heads + kvh) * a.page_tokens + (box - idx * page_boxes) * box_rows
+                   : none;
+      };
+      auto load = [&](const CUtensorMap& map, int slot, int row) {
+        if (lane == 0) mbar_arrive_expect_tx(&full[slot], S::kTile);
+        __syncwarp();
+        if (lane < boxes) {
 #pragma unroll
-              for (int h = 0; h < D / 64; ++h) {
-                uint8_t* to = dst + h * S::kHalf + x * box_rows * 128;
-                // (two calls: a selected pointer would make the compiler copy the maps to the stack)
-                if (kv)
-                  tma_load_2d(to, &tm_v, &full[st], h * 64, row);
-                else
-                  tma_load_2d(to, &tm_k, &full[st], h * 64, row);
-              }
-            }
-          }
+          for (int h = 0; h < D / 64; ++h)
+            tma_load_2d(ring + slot * S::kTile + lane * box_rows * 128 + h * S::kHalf, &map, &full[slot], h * 64, row);
         }
-        if (!ok)  // gave up: let the copies in flight land before the memory is given back
-          for (int i = max(0, it - kStages); i < it; ++i) mbar_wait(&full[i % kStages], (i / kStages) & 1);
-      }
-    } else if (warp == 8) {
-      if (lane == 0) {
-        // ------------------------------------------------------------ MMA
-        constexpr uint32_t idesc_s = umma_idesc<T>(kWtRows, kWtKeys, false);
-        constexpr uint32_t idesc_o = umma_idesc<T>(kWtRows, D, true);
-        const uint32_t q_addr = smem_u32(sQ), ring_addr = smem_u32(ring);
-        auto qk = [&](int i, int st) {
-          const uint32_t qa = q_addr + i * S::kTile, ka = ring_addr + st * S::kTile;
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            umma_bf16(tmem + i * 128, umma_desc_sw128(qa + (k >> 2) * S::kHalf + (k & 3) * 32),
-                      umma_desc_sw128(ka + (k >> 2) * S::kHalf + (k & 3) * 32), idesc_s, k > 0);
-          umma_commit(&s_full[i]);
-        };
-        auto pv = [&](int i, int st, bool acc) {
-          const uint32_t va = ring_addr + st * S::kTile;
-#pragma unroll
-          for (int k = 0; k < kWtKeys / 16; ++k)
-            umma_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8,
-                    wt_v_desc(va + k * 2048), idesc_o, acc || k > 0);
-          umma_commit(&pv_done[i]);
-        };
-        bool ok = mbar_wait(q_full, 0);
-        uint32_t np[2] = {0, 0};  // P tiles taken
-        if (ok && n > 0) {
-          const int t0 = tiles.tile(0) * kWtKeys;
-          ok = mbar_wait(&full[0], 0);
-          if (ok) {
-            tc_fence_after();
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (half[i].some(t0, t0 + kWtKeys)) qk(i, 0);
-            umma_commit(&empty[0]);
-          }
-        }
-        for (int j = 0; j < n && ok; ++j) {
-          const int k0 = tiles.tile(j) * kWtKeys, k1 = j + 1 < n ? tiles.tile(j + 1) * kWtKeys : 0;
-          const int vi = 2 * j + 1, ki = 2 * j + 2;
-          const int vs = vi % kStages, ks = ki % kStages;
-          ok = mbar_wait(&clean[vs], (vi / kStages) & 1);
-          if (ok && j + 1 < n) ok = mbar_wait(&full[ks], (ki / kStages) & 1);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (half[i].some(k0, k0 + kWtKeys)) {
-              ok = ok && mbar_wait(&p_full[i], np[i] & 1);
-              if (!ok) break;
-              tc_fence_after();
-              pv(i, vs, np[i] > 0);
-              ++np[i];
-            }
-            if (j + 1 < n && half[i].some(k1, k1 + kWtKeys)) qk(i, ks);
-          }
-          if (!ok) break;
-          umma_commit(&empty[vs]);
-          if (j + 1 < n) umma_commit(&empty[ks]);
-        }
-      }
-    } else {
-      // -------------------------------------------------------------- V tiles seen in part
-      // Zeroes the rows that no query of this CTA sees (ends of pages, tokens before the window):
-      // their weights are 0, but 0 * NaN is not.  An infinity or NaN in a row that only some of
-      // the queries see marks the CTA: its rows are then computed one by one (window_row).
-      const int w = warp - 10;
-      bool ok = true;
-      for (int j = 0; j < n && ok; ++j) {
-        const int vi = 2 * j + 1, st = vi % kStages;
+        __syncwarp();
+      };
+      auto look_over = [&](int j) {
+        const int st = kSK + j % kSV;
         const int k0 = tiles.tile(j) * kWtKeys;
-        ok = mbar_wait(&full[st], (vi / kStages) & 1);
-        if (ok && !span.all(k0, k0 + kWtKeys)) {
+        bool ok = true;
+        if (!span.all(k0, k0 + kWtKeys)) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&full[st], (j / kSV) & 1));
           uint8_t* v = ring + st * S::kTile;
           bool bad = false;
-          for (int r = w * (kWtKeys / 2) + lane / 8; r < (w + 1) * (kWtKeys / 2); r += 4) {
+          for (int r = lane / 8; ok && r < kWtKeys; r += 4) {
             const bool seen = span.sees(k0 + r);
 #pragma unroll
             for (int h = 0; h < D / 64; ++h) {
@@ -404,10 +353,95 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&clean[st]);
+        return ok;
+      };
+      int nk = 0, nv = 0;  // tiles asked for
+      for (; nv < min(n, kSV); ++nv) {
+        const int row = box_row(nv);
+        if (nv < kSK) load(tm_k, nk++, row);
+        load(tm_v, kSK + nv, row);
+      }
+      bool ok = n == 0 || look_over(0);
+      for (int j = 0; j < n && ok; ++j) {
+        if (nk < n) {
+          const int row = box_row(nk);
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[j % kSK], (j / kSK) & 1));
+          if (ok) load(tm_k, nk++ % kSK, row);
+        }
+        if (ok && j + 1 < n) ok = look_over(j + 1);
+        if (ok && nv < n) {
+          const int row = box_row(nv);
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[kSK + j % kSV], (j / kSV) & 1));
+          if (ok) load(tm_v, kSK + nv++ % kSV, row);
+        }
+      }
+      if (!ok) {  // gave up: let the copies in flight land before the memory is given back
+        for (int j = max(0, nk - kSK); j < nk; ++j) mbar_wait(&full[j % kSK], (j / kSK) & 1);
+        for (int j = max(0, nv - kSV); j < nv; ++j) mbar_wait(&full[kSK + j % kSV], (j / kSV) & 1);
+      }
+    } else {
+      if (lane == 0) {
+        // ------------------------------------------------------------ MMA
+        constexpr uint32_t idesc_s = umma_idesc<T>(kWtRows, kWtKeys, false);
+        constexpr uint32_t idesc_o = umma_idesc<T>(kWtRows, D, true);
+        const uint32_t q_addr = smem_u32(sQ), ring_addr = smem_u32(ring);
+        auto qk = [&](int i, int st) {
+          const uint32_t qa = q_addr + i * S::kTile, ka = ring_addr + st * S::kTile;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_bf16(tmem + i * 128, umma_desc_sw128(qa + (k >> 2) * S::kHalf + (k & 3) * 32),
+                      umma_desc_sw128(ka + (k >> 2) * S::kHalf + (k & 3) * 32), idesc_s, k > 0);
+          umma_commit(&s_full[i]);
+        };
+        auto pv = [&](int i, int st, int k0, bool acc) {  // half of the keys
+          const uint32_t va = ring_addr + st * S::kTile;
+#pragma unroll
+          for (int k = k0; k < k0 + kWtKeys / 32; ++k)
+            umma_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8, wt_v_desc(va + k * 2048), idesc_o, acc || k > k0);
+        };
+        bool ok = mbar_wait(q_full, 0);
+        uint32_t np[2] = {0, 0};  // P tiles taken
+        if (ok && n > 0) {
+          const int t0 = tiles.tile(0) * kWtKeys;
+          ok = mbar_wait(&full[0], 0);
+          if (ok) {
+            tc_fence_after();
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (half[i].some(t0, t0 + kWtKeys)) qk(i, 0);
+            umma_commit(&empty[0]);
+          }
+        }
+        for (int j = 0; j < n && ok; ++j) {
+          const int k0 = tiles.tile(j) * kWtKeys, k1 = j + 1 < n ? tiles.tile(j + 1) * kWtKeys : 0;
+          const int vs = kSK + j % kSV, ks = (j + 1) % kSK;
+          ok = mbar_wait(&full[vs], (j / kSV) & 1) && mbar_wait(&clean[vs], (j / kSV) & 1);
+          if (ok && j + 1 < n) ok = mbar_wait(&full[ks], ((j + 1) / kSK) & 1);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (half[i].some(k0, k0 + kWtKeys)) {
+              ok = ok && mbar_wait(&p_half[i], np[i] & 1);
+              if (!ok) break;
+              tc_fence_after();
+              pv(i, vs, 0, np[i] > 0);
+              ok = mbar_wait(&p_full[i], np[i] & 1);
+              if (!ok) break;
+              tc_fence_after();
+              pv(i, vs, kWtKeys / 32, true);
+              umma_commit(&pv_done[i]);
+              ++np[i];
+            }
+            if (j + 1 < n && half[i].some(k1, k1 + kWtKeys)) qk(i, ks);
+          }
+          if (!ok) break;
+          umma_commit(&empty[vs]);
+          if (j + 1 < n) umma_commit(&empty[ks]);
+        }
       }
     }
   } else {
-    reg_inc<208>();
     if (row0 < rows) {
       // -------------------------------------------------------------- softmax
       const int i = warp >> 2;                  // tile
@@ -440,70 +474,61 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       const uint32_t s_addr = tmem + i * 128 + (static_cast<uint32_t>(quarter * 32) << 16);
       const uint32_t o_addr = tmem + 256 + i * D + (static_cast<uint32_t>(quarter * 32) << 16);
       const float sl2 = a.scale_log2;
-      const int boxes = kWtKeys / box_rows, page_boxes = a.page_tokens / box_rows;
+      // whether some page in sight is not there: only then are the tiles' pages looked up
+      bool hole = false;
+      for (int j = 0; j < 2; ++j) {
+        const int p0 = j ? mine.lo.start / a.page_tokens : 0;
+        const int p1 = ((j ? mine.hi.end : mine.hi.sink_end) + a.page_tokens - 1) / a.page_tokens;
+        for (int x = p0 + lane; x < p1; x += 32) hole = hole || table[x] < 0 || table[x] >= a.pages;
+      }
+      const bool holes = __any_sync(0xffffffffu, hole && mine.any);
       float m = -INFINITY, l = 0.0f;
       uint32_t np = 0;
       bool ok = true;
       for (int j = 0; j < n; ++j) {
         const int tile = tiles.tile(j), k0 = tile * kWtKeys;
         if (!mine.some(k0, k0 + kWtKeys)) continue;
-        // pages that are not there (before the wait: the look-up runs under it)
-        bool hole = false;
-        if (lane < boxes) {
-          const int idx = (tile * boxes + lane) / page_boxes;
-          const int page = idx < a.width ? table[idx] : -1;
-          hole = page < 0 || page >= a.pages;
-        }
-        const uint32_t holes = __ballot_sync(0xffffffffu, hole);
         ok = mbar_wait(&s_full[i], np & 1);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
-        // S twice through 32 columns at a time (maximum, then weights): half the registers of
-        // holding the row, and TMEM reads are cheap beside the exponentials
         const bool part = holes || !mine.all(k0, k0 + kWtKeys);
-        uint32_t seen[4] = {~0u, ~0u, ~0u, ~0u};
+        uint32_t v[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32_nowait(s_addr + c * 32, v[c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_wait_ld(v[c]);
         if (part) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int k = k0 + c * 32;
-            seen[c] = wt_bits(range.start - k, range.end - k) | wt_bits(-k, range.sink_end - k);
+            uint32_t seen = wt_bits(range.start - k, range.end - k) | wt_bits(-k, range.sink_end - k);
             if (holes) {
 #pragma unroll
-              for (int x = 0; x < 32; x += 16)
-                if ((holes >> ((c * 32 + x) / box_rows)) & 1u) seen[c] &= ~(0xffffu << x);
+              for (int x = 0; x < 32; x += 16) {  // a page is a multiple of 16 tokens
+                const int idx = (k + x) / a.page_tokens;
+                const int page = idx < a.width ? table[idx] : -1;
+                if (page < 0 || page >= a.pages) seen &= ~(0xffffu << x);
+              }
             }
+            wt_hide(v[c], seen);
           }
         }
-        uint32_t sa[32], sb[32];
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        auto maxima = [&](uint32_t(&v)[32], uint32_t bits) {
-          if (part) wt_hide(v, bits);
 #pragma unroll
-          for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(v[x]));
-        };
-        tmem_ld32_nowait(s_addr, sa);
-        tmem_wait_ld(sa);
-        tmem_ld32_nowait(s_addr + 32, sb);
-        maxima(sa, seen[0]);
-        tmem_wait_ld(sb);
-        tmem_ld32_nowait(s_addr + 64, sa);
-        maxima(sb, seen[1]);
-        tmem_wait_ld(sa);
-        tmem_ld32_nowait(s_addr + 96, sb);
-        maxima(sa, seen[2]);
-        tmem_wait_ld(sb);
-        tmem_ld32_nowait(s_addr, sa);
-        maxima(sb, seen[3]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        // -inf - -inf is NaN and compares false: nothing seen yet keeps m
-        const bool grow = (top - m) * sl2 > kWtLazy;
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int x = 0; x < 32; x += 2)
+            mx[(x >> 1) & 3] = max3_nan(mx[(x >> 1) & 3], __uint_as_float(v[c][x]), __uint_as_float(v[c][x + 1]));
+        const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+        // a NaN score makes the maximum and with it the whole row NaN; a tile without a visible
+        // key (top -inf) changes nothing
+        const bool grow = !((top - m) * sl2 <= kWtLazy) && top != -INFINITY;
         float alpha = 1.0f;
         if (grow) {
           alpha = ex2((m - top) * sl2);  // 0 at the first tile
           m = top;
           l *= alpha;
         }
-        tmem_wait_ld(sa);
         if (np > 0 && __any_sync(0xffffffffu, grow)) {
           ok = mbar_wait(&pv_done[i], (np - 1) & 1);
           if (!__all_sync(0xffffffffu, ok)) break;
@@ -518,33 +543,41 @@ __global__ void __launch_bounds__(kWtThreads, 1)
             tmem_st32(o_addr + c * 32, o);
           }
         }
-        const float base = m == -INFINITY ? 0.0f : -m * sl2;
+        const float base = m == -INFINITY ? 0.0f : fmaf(m, 0.0f, -m * sl2);  // NaN for a maximum of +inf
         uint64_t sum[2] = {0, 0};
-        // the columns of P lie over columns of S that have been read
-        auto weights = [&](uint32_t(&v)[32], uint32_t bits, int c) {
-          if (part) wt_hide(v, bits);
-          uint32_t pk[16];
+        // the columns of P lie over those of S, which are all in registers; the MMAs take the
+        // first half of the keys while the second is computed
+        auto weights = [&](auto partial) {
+          constexpr bool PART = decltype(partial)::value;
 #pragma unroll
-          for (int x = 0; x < 32; x += 2) {
-            const uint64_t t = fma_f32x2(pair_f32(v[x], v[x + 1]), pair_f32(sl2, sl2), pair_f32(base, base));
-            float2 e = unpair_f32(t);
-            e.x = ex2(e.x);
-            e.y = ex2(e.y);
-            sum[(x >> 1) & 1] = add_f32x2(sum[(x >> 1) & 1], pair_f32(e.x, e.y));
-            pk[x / 2] = pack2<T>(e.x, e.y);
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int x = 0; x < 32; x += 2) {
+              const uint64_t t = fma_f32x2(pair_f32(v[c][x], v[c][x + 1]), pair_f32(sl2, sl2), pair_f32(base, base));
+              float2 e = unpair_f32(t);
+              if (!PART && (x >> 1) % kWtPolyEvery == kWtPolyEvery - 1) {
+                e = exp2_poly(t);
+              } else {
+                e.x = ex2(e.x);
+                e.y = ex2(e.y);
+              }
+              sum[(x >> 1) & 1] = add_f32x2(sum[(x >> 1) & 1], pair_f32(e.x, e.y));
+              pk[x / 2] = pack2<T>(e.x, e.y);
+            }
+            tmem_st16(s_addr + c * 16, pk);
+            if (c == 1) {
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_half[i]);
+            }
           }
-          tmem_st16(s_addr + c * 16, pk);
         };
-        tmem_ld32_nowait(s_addr + 32, sb);
-        weights(sa, seen[0], 0);
-        tmem_wait_ld(sb);
-        tmem_ld32_nowait(s_addr + 64, sa);
-        weights(sb, seen[1], 1);
-        tmem_wait_ld(sa);
-        tmem_ld32_nowait(s_addr + 96, sb);
-        weights(sa, seen[2], 2);
-        tmem_wait_ld(sb);
-        weights(sb, seen[3], 3);
+        if (part)
+          weights(std::true_type{});
+        else
+          weights(std::false_type{});
         const float2 s2 = unpair_f32(add_f32x2(sum[0], sum[1]));
         l += s2.x + s2.y;
         tmem_wait_st();
@@ -556,7 +589,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       if (ok && np > 0) ok = mbar_wait(&pv_done[i], (np - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      // the V warps' mark: every tile they looked at was multiplied before pv_done
+      // warp 9's mark: every tile it looked at was multiplied before pv_done
       if (ok && *reinterpret_cast<volatile uint32_t*>(dirty)) {
         for (int x = 0; x < 32; ++x) {
           const int rr = row0 + i * kWtRows + quarter * 32 + x;
