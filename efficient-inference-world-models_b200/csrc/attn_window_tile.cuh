@@ -44,15 +44,32 @@ __device__ __forceinline__ uint64_t wt_v_desc(uint32_t smem_addr) {
   return d;
 }
 
-// P (A operand, K-major) from TMEM, V (B operand) from shared memory.
+// D (+)= A B^T with A from shared memory, and with A (P, K-major) from TMEM.
+__device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
                                         uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 
 // 32 columns of this warp's 32 lanes, not waited for.
@@ -257,7 +274,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
   uint32_t* dirty = tmem_holder + 1;
 
   pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 1);
@@ -380,65 +397,88 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         for (int j = max(0, nv - kSV); j < nv; ++j) mbar_wait(&full[kSK + j % kSV], (j / kSV) & 1);
       }
     } else {
-      if (lane == 0) {
-        // ------------------------------------------------------------ MMA
-        constexpr uint32_t idesc_s = umma_idesc<T>(kWtRows, kWtKeys, false);
-        constexpr uint32_t idesc_o = umma_idesc<T>(kWtRows, D, true);
-        const uint32_t q_addr = smem_u32(sQ), ring_addr = smem_u32(ring);
-        auto qk = [&](int i, int st) {
-          const uint32_t qa = q_addr + i * S::kTile, ka = ring_addr + st * S::kTile;
+      // -------------------------------------------------------------- MMA: one lane issues, the
+      // warp stays converged, so that descriptors are warp-uniform values
+      constexpr uint32_t idesc_s = umma_idesc<T>(kWtRows, kWtKeys, false);
+      constexpr uint32_t idesc_o = umma_idesc<T>(kWtRows, D, true);
+      const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ)), k_desc = umma_desc_sw128(smem_u32(ring));
+      const uint64_t v_desc = wt_v_desc(smem_u32(ring));
+      constexpr uint64_t kTile16 = S::kTile >> 4, kHalf16 = S::kHalf >> 4;
+      auto qk = [&](int i, int st) {
+        const uint64_t qa = q_desc + i * kTile16, ka = k_desc + st * kTile16;
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            umma_bf16(tmem + i * 128, umma_desc_sw128(qa + (k >> 2) * S::kHalf + (k & 3) * 32),
-                      umma_desc_sw128(ka + (k >> 2) * S::kHalf + (k & 3) * 32), idesc_s, k > 0);
-          umma_commit(&s_full[i]);
-        };
-        auto pv = [&](int i, int st, int k0, bool acc) {  // half of the keys
-          const uint32_t va = ring_addr + st * S::kTile;
+        for (int k = 0; k < D / 16; ++k)
+          umma_ss(tmem + i * 128, qa + (k >> 2) * kHalf16 + (k & 3) * 2, ka + (k >> 2) * kHalf16 + (k & 3) * 2, idesc_s,
+                  k > 0);
+      };
+      auto pv = [&](int i, int st, int k0, uint32_t acc) {  // half of the keys
+        const uint64_t va = v_desc + st * kTile16;
 #pragma unroll
-          for (int k = k0; k < k0 + kWtKeys / 32; ++k)
-            umma_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8, wt_v_desc(va + k * 2048), idesc_o, acc || k > k0);
-        };
-        bool ok = mbar_wait(q_full, 0);
-        uint32_t np[2] = {0, 0};  // P tiles taken
-        if (ok && n > 0) {
-          const int t0 = tiles.tile(0) * kWtKeys;
-          ok = mbar_wait(&full[0], 0);
-          if (ok) {
-            tc_fence_after();
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (half[i].some(t0, t0 + kWtKeys)) qk(i, 0);
-            umma_commit(&empty[0]);
+        for (int k = k0; k < k0 + kWtKeys / 32; ++k)
+          umma_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8, va + k * 128, idesc_o, k == k0 ? acc : 1u);
+      };
+      bool ok = mbar_wait(q_full, 0);
+      uint32_t np0 = 0, np1 = 0;  // P tiles taken
+      if (n > 0) {
+        const int t0 = tiles.tile(0) * kWtKeys;
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(&full[0], 0));
+        tc_fence_after();
+        if (ok && elect_one()) {
+          if (half[0].some(t0, t0 + kWtKeys)) {
+            qk(0, 0);
+            umma_commit(&s_full[0]);
           }
+          if (half[1].some(t0, t0 + kWtKeys)) {
+            qk(1, 0);
+            umma_commit(&s_full[1]);
+          }
+          umma_commit(&empty[0]);
         }
-        for (int j = 0; j < n && ok; ++j) {
-          const int k0 = tiles.tile(j) * kWtKeys, k1 = j + 1 < n ? tiles.tile(j + 1) * kWtKeys : 0;
-          const int vs = kSK + j % kSV, ks = (j + 1) % kSK;
-          ok = mbar_wait(&full[vs], (j / kSV) & 1) && mbar_wait(&clean[vs], (j / kSV) & 1);
-          if (ok && j + 1 < n) ok = mbar_wait(&full[ks], ((j + 1) / kSK) & 1);
-          if (!ok) break;
+        __syncwarp();
+      }
+      // PV_i(j), then QK_i(j+1)
+      auto turn = [&](int i, uint32_t& np, bool now, bool next, int vs, int ks) {
+        if (now) {
+          ok = __all_sync(0xffffffffu, ok && mbar_wait(&p_half[i], np & 1));
+          if (!ok) return;
           tc_fence_after();
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (half[i].some(k0, k0 + kWtKeys)) {
-              ok = ok && mbar_wait(&p_half[i], np[i] & 1);
-              if (!ok) break;
-              tc_fence_after();
-              pv(i, vs, 0, np[i] > 0);
-              ok = mbar_wait(&p_full[i], np[i] & 1);
-              if (!ok) break;
-              tc_fence_after();
-              pv(i, vs, kWtKeys / 32, true);
-              umma_commit(&pv_done[i]);
-              ++np[i];
-            }
-            if (j + 1 < n && half[i].some(k1, k1 + kWtKeys)) qk(i, ks);
+          if (elect_one()) pv(i, vs, 0, np > 0);
+          __syncwarp();
+          ok = __all_sync(0xffffffffu, mbar_wait(&p_full[i], np & 1));
+          if (!ok) return;
+          tc_fence_after();
+          if (elect_one()) {
+            pv(i, vs, kWtKeys / 32, 1u);
+            umma_commit(&pv_done[i]);
           }
-          if (!ok) break;
-          umma_commit(&empty[vs]);
-          if (j + 1 < n) umma_commit(&empty[ks]);
+          __syncwarp();
+          ++np;
         }
+        if (next) {
+          if (elect_one()) {
+            qk(i, ks);
+            umma_commit(&s_full[i]);
+          }
+          __syncwarp();
+        }
+      };
+      for (int j = 0; j < n && ok; ++j) {
+        const int k0 = tiles.tile(j) * kWtKeys, k1 = j + 1 < n ? tiles.tile(j + 1) * kWtKeys : 0;
+        const bool more = j + 1 < n;
+        const int vs = kSK + j % kSV, ks = (j + 1) % kSK;
+        ok = mbar_wait(&full[vs], (j / kSV) & 1) && mbar_wait(&clean[vs], (j / kSV) & 1);
+        if (ok && more) ok = mbar_wait(&full[ks], ((j + 1) / kSK) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        turn(0, np0, half[0].some(k0, k0 + kWtKeys), more && half[0].some(k1, k1 + kWtKeys), vs, ks);
+        turn(1, np1, half[1].some(k0, k0 + kWtKeys), more && half[1].some(k1, k1 + kWtKeys), vs, ks);
+        if (!ok) break;
+        if (elect_one()) {
+          umma_commit(&empty[vs]);
+          if (more) umma_commit(&empty[ks]);
+        }
+        __syncwarp();
       }
     }
   } else {
