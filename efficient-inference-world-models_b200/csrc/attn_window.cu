@@ -122,19 +122,10 @@ __device__ __noinline__ void window_row(const WinArgs& a, int b, const WinSeq& s
     a.lse[row * a.heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(128) attn_window_rows_kernel(const __grid_constant__ WinArgs a) {
-  pdl_trigger();
-  pdl_wait();
-  const int b = blockIdx.z, lane = threadIdx.x & 31;
-  const WinSeq s = win_seq(a, b);
-  for (int qi = blockIdx.x * 4 + (threadIdx.x >> 5); qi < s.n_q; qi += gridDim.x * 4)
-    window_row<T, D>(a, b, s, qi, blockIdx.y, lane);
-}
-
 }  // namespace oasis
 
 #include "attn_window_tile.cuh"
+#include "attn_window_few.cuh"
 
 namespace oasis {
 
@@ -168,6 +159,25 @@ int encode_page_rows(CUtensorMap* map, const void* base, const WinArgs& a, int d
   return encode_bf16_sw128(map, base, 2, dims, strides, box);
 }
 
+// Keys of the longest sequence that a query can see under the window.
+inline long long visible_keys(const WinArgs& a, int max_kv) {
+  if (!a.window) return max_kv;
+  return std::min<long long>(max_kv, (static_cast<long long>(a.window) + a.sinks) * a.frame);
+}
+
+template <typename T, int D, int NR>
+int launch_attn_window_few(const WinArgs& a, int max_kv, cudaStream_t stream) {
+  // CTAs per (sequence, key head): enough for four full waves, while a warp keeps 8 steps of 16 keys
+  const long long base = static_cast<long long>(a.batch) * a.kv_heads;
+  const long long steps = (visible_keys(a, max_kv) + 15) / 16;
+  int splits = 1;
+  while (splits < 8 && base * splits < 12LL * num_sms() && steps > splits * kFewWarps) splits *= 2;
+  cudaError_t e = launch_pdl_cluster(attn_window_few_kernel<T, D, NR>, dim3(splits * a.kv_heads, 1, a.batch),
+                                     dim3(kFewWarps * 32), 0, stream, splits, a, splits);
+  if (e != cudaSuccess) return cuda_status(e, "attn_window_few_kernel");
+  return OASIS_OK;
+}
+
 template <typename T, int D>
 int launch_attn_window(const WinArgs& a, int max_q, int max_kv, cudaStream_t stream) {
   const long long max_rows = static_cast<long long>(max_q) * a.group;
@@ -183,10 +193,8 @@ int launch_attn_window(const WinArgs& a, int max_q, int max_kv, cudaStream_t str
     if (e != cudaSuccess) return cuda_status(e, "attn_window_tile_kernel");
     return OASIS_OK;
   }
-  cudaError_t e = launch_pdl(attn_window_rows_kernel<T, D>, dim3((max_q + 3) / 4, a.heads, a.batch), dim3(128), 0,
-                             stream, a);
-  if (e != cudaSuccess) return cuda_status(e, "attn_window_rows_kernel");
-  return OASIS_OK;
+  return max_rows <= 8 ? launch_attn_window_few<T, D, 8>(a, max_kv, stream)
+                       : launch_attn_window_few<T, D, 16>(a, max_kv, stream);
 }
 
 }  // namespace oasis

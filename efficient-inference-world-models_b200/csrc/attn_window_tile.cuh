@@ -574,13 +574,13 @@ __global__ void __launch_bounds__(kWtThreads, 1)
           if (!__all_sync(0xffffffffu, ok)) break;
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32_nowait(o_addr + c * 32, o);
-            tmem_wait_ld(o);
+          for (int c = 0; c < D / 16; ++c) {  // few columns at a time: the row of S stays in registers
+            float o[16];
+            tmem_ld16(o_addr + c * 16, o);
+            uint32_t w[16];
 #pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
-            tmem_st32(o_addr + c * 32, o);
+            for (int x = 0; x < 16; ++x) w[x] = __float_as_uint(o[x] * alpha);
+            tmem_st16(o_addr + c * 16, w);
           }
         }
         const float base = m == -INFINITY ? 0.0f : fmaf(m, 0.0f, -m * sl2);  // NaN for a maximum of +inf
