@@ -41,6 +41,8 @@ __device__ __forceinline__ WinSeq win_seq(const WinArgs& a, int b) {
   return s;
 }
 
+constexpr int kWinSplits = 8;  // CTAs of a cluster, at most: the portable size
+
 struct WinRange {
   int sink_end, start, end;  // visible: [0, sink_end) and [start, end); sink_end <= start
   __device__ __forceinline__ bool sees(int key) const {
@@ -71,6 +73,20 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 from_float(float x) { return __float2bfloat16_rn(x); }
 template <>
 __device__ __forceinline__ __half from_float(float x) { return __float2half_rn(x); }
+
+// From the shared memory of a CTA of the cluster (a mapa_shared address).
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr));
+  return v;
+}
 
 // One query row by one warp, key after key with the running maximum and sum: each lane holds
 // D / 32 dims.  Reads only what the row sees.
@@ -165,13 +181,32 @@ inline long long visible_keys(const WinArgs& a, int max_kv) {
   return std::min<long long>(max_kv, (static_cast<long long>(a.window) + a.sinks) * a.frame);
 }
 
+// CTAs of a cluster that share the keys of one pair of query tiles: the count of least estimated
+// time, where a CTA costs its key tiles and about 3 more to begin and end, joining 2 more, and
+// a wave is one CTA per SM (clusters of 8 fill 128 SMs: they lie within a GPC).
+inline int tile_splits(long long pairs, long long keys) {
+  const long long tiles = (keys + kWtKeys - 1) / kWtKeys;
+  int best = 1;
+  double least = 0.0;
+  for (int s = 1; s <= kWinSplits; s *= 2) {
+    const long long sms = s == 8 ? 128 : num_sms() / s * s;
+    const double cost = static_cast<double>((pairs * s + sms - 1) / sms) *
+                        (static_cast<double>((tiles + s - 1) / s) + 3.0 + (s > 1 ? 2.0 : 0.0));
+    if (s == 1 || cost < least) {
+      best = s;
+      least = cost;
+    }
+  }
+  return best;
+}
+
 template <typename T, int D, int NR>
 int launch_attn_window_few(const WinArgs& a, int max_kv, cudaStream_t stream) {
   // CTAs per (sequence, key head): enough for four full waves, while a warp keeps 8 steps of 16 keys
   const long long base = static_cast<long long>(a.batch) * a.kv_heads;
   const long long steps = (visible_keys(a, max_kv) + 15) / 16;
   int splits = 1;
-  while (splits < 8 && base * splits < 12LL * num_sms() && steps > splits * kFewWarps) splits *= 2;
+  while (splits < kWinSplits && base * splits < 12LL * num_sms() && steps > splits * kFewWarps) splits *= 2;
   cudaError_t e = launch_pdl_cluster(attn_window_few_kernel<T, D, NR>, dim3(splits * a.kv_heads, 1, a.batch),
                                      dim3(kFewWarps * 32), 0, stream, splits, a, splits);
   if (e != cudaSuccess) return cuda_status(e, "attn_window_few_kernel");
@@ -188,8 +223,12 @@ int launch_attn_window(const WinArgs& a, int max_q, int max_kv, cudaStream_t str
     if (int st = encode_page_rows(&tv, a.v, a, D, box)) return st;
     if (int st = allow_smem<attn_window_tile_kernel<T, D>>(WtShape<D>::kSmem, "attn_window_tile_kernel")) return st;
     const int row_tiles = static_cast<int>((max_rows + 2 * kWtRows - 1) / (2 * kWtRows));
-    cudaError_t e = launch_pdl(attn_window_tile_kernel<T, D>, dim3(row_tiles * a.kv_heads, 1, a.batch),
-                               dim3(kWtThreads), WtShape<D>::kSmem, stream, a, tk, tv, box, row_tiles);
+    const int splits = tile_splits(static_cast<long long>(row_tiles) * a.kv_heads * a.batch, visible_keys(a, max_kv));
+    if (static_cast<long long>(row_tiles) * a.kv_heads * splits > 0x7fffffffLL)
+      return fail(OASIS_ERR_UNSUPPORTED, "oasis_attn_window: too many query rows");
+    cudaError_t e = launch_pdl_cluster(attn_window_tile_kernel<T, D>, dim3(row_tiles * a.kv_heads * splits, 1, a.batch),
+                                       dim3(kWtThreads), WtShape<D>::kSmem, stream, splits, a, tk, tv, box, row_tiles,
+                                       splits);
     if (e != cudaSuccess) return cuda_status(e, "attn_window_tile_kernel");
     return OASIS_OK;
   }

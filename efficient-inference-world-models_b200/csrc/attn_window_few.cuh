@@ -41,20 +41,6 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
   return v;
 }
 
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
-
 template <int D, int NR>
 struct alignas(16) FewShared {
   float o[kFewWarps][NR][D];
@@ -325,20 +311,29 @@ __global__ void __launch_bounds__(kFewWarps * 32, D == 64 ? (NR == 8 ? 4 : 3) : 
     else
       __syncthreads();
     uint32_t marked = 0;
-    for (int x = 0; x < splits; ++x)
-      marked |= __float_as_uint(ld_cluster(mapa_shared(smem_u32(&sh.dirty), x)));
+#pragma unroll
+    for (int x = 0; x < kWinSplits; ++x)
+      if (x < splits) marked |= __float_as_uint(ld_cluster(mapa_shared(smem_u32(&sh.dirty), x)));
     if (marked) {
       for (int r = row0 + part; r < row1; r += parts)
         window_row<T, D>(a, b, seq, r / a.group, kvh * a.group + r % a.group, lane);
     } else {
       for (int e = split * kFewWarps * 32 + threadIdx.x; e < (row1 - row0) * (D / 4); e += splits * kFewWarps * 32) {
         const int r = e / (D / 4), d = (e % (D / 4)) * 4;
-        float top = -INFINITY;
-        for (int x = 0; x < splits; ++x) top = join_max(top, ld_cluster(mapa_shared(smem_u32(&sh.cm[r]), x)));
+        float mx[kWinSplits], top = -INFINITY;  // all loads in flight at once
+#pragma unroll
+        for (int x = 0; x < kWinSplits; ++x) {
+          mx[x] = -INFINITY;
+          if (x < splits) mx[x] = ld_cluster(mapa_shared(smem_u32(&sh.cm[r]), x));
+        }
+#pragma unroll
+        for (int x = 0; x < kWinSplits; ++x) top = join_max(top, mx[x]);
         float sum = 0.0f;
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int x = 0; x < splits; ++x) {
-          const float f = weight(ld_cluster(mapa_shared(smem_u32(&sh.cm[r]), x)), top);
+#pragma unroll
+        for (int x = 0; x < kWinSplits; ++x) {
+          if (x >= splits) continue;
+          const float f = weight(mx[x], top);
           const float4 z = ld_cluster4(mapa_shared(smem_u32(&sh.o[0][r][d]), x));
           sum += f * ld_cluster(mapa_shared(smem_u32(&sh.cl[r]), x));
           acc.x = fmaf(f, z.x, acc.x), acc.y = fmaf(f, z.y, acc.y);

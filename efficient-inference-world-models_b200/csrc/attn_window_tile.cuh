@@ -241,11 +241,18 @@ __device__ __forceinline__ WtSpan wt_span(const WinArgs& a, const WinSeq& s, int
 
 // The key tiles of a span: [0, sink) and [first, last).
 struct WtTiles {
-  int sink, first, n;
-  __device__ __forceinline__ int tile(int j) const { return j < sink ? j : first + j - sink; }
+  int sink, first, n, skip;
+  __device__ __forceinline__ int tile(int j) const { return j < sink ? skip + j : first + j - sink; }
+  // The part of them that CTA `rank` of `parts` takes, numbered from 0.
+  __device__ __forceinline__ void keep(int rank, int parts) {
+    const int j0 = n * rank / parts, j1 = n * (rank + 1) / parts;
+    sink -= j0;  // negative: all of the part lies in the window
+    skip = j0;
+    n = j1 - j0;
+  }
 };
 __device__ __forceinline__ WtTiles wt_tiles(const WtSpan& w, int keys) {
-  WtTiles t = {0, 0, 0};
+  WtTiles t = {0, 0, 0, 0};
   if (!w.any) return t;
   t.sink = (min(w.hi.sink_end, w.lo.start) + keys - 1) / keys;
   t.first = max(w.lo.start / keys, t.sink);
@@ -256,7 +263,7 @@ __device__ __forceinline__ WtTiles wt_tiles(const WtSpan& w, int keys) {
 template <typename T, int D>
 __global__ void __launch_bounds__(kWtThreads, 1)
     attn_window_tile_kernel(const __grid_constant__ WinArgs a, const __grid_constant__ CUtensorMap tm_k,
-                            const __grid_constant__ CUtensorMap tm_v, int box_rows, int row_tiles) {
+                            const __grid_constant__ CUtensorMap tm_v, int box_rows, int row_tiles, int splits) {
   using S = WtShape<D>;
   constexpr int kStages = S::kStages, kSK = S::kStagesK, kSV = S::kStagesV;  // slots: K, then V
   extern __shared__ uint8_t wt_raw[];
@@ -304,16 +311,25 @@ __global__ void __launch_bounds__(kWtThreads, 1)
   const WinSeq seq = win_seq(a, b);
   const int rows = seq.n_q * a.group;
   // later rows of a causal prompt see more: they start first
-  const int tile_id = row_tiles - 1 - static_cast<int>(blockIdx.x) / a.kv_heads;
-  const int kvh = static_cast<int>(blockIdx.x) % a.kv_heads;
+  const int rank = static_cast<int>(blockIdx.x) % splits;  // in the cluster, which shares the keys
+  const int unit = static_cast<int>(blockIdx.x) / splits;
+  const int tile_id = row_tiles - 1 - unit / a.kv_heads;
+  const int kvh = unit % a.kv_heads;
   const int row0 = tile_id * (2 * kWtRows);
   const int32_t* table = a.table + static_cast<long long>(b) * a.width;
   const int row1 = min(rows, row0 + 2 * kWtRows);
   const WtSpan span = wt_span(a, seq, row0, row1);
   const WtSpan half[2] = {wt_span(a, seq, row0, min(row1, row0 + kWtRows)),
                           wt_span(a, seq, min(row1, row0 + kWtRows), row1)};
-  const WtTiles tiles = wt_tiles(span, kWtKeys);
+  WtTiles tiles = wt_tiles(span, kWtKeys);
+  tiles.keep(rank, splits);
   const int n = tiles.n;
+  // a split CTA's result, over the ring once it is done: O [256][D] fp32 (16-byte chunks
+  // swizzled by row), then the rows' maxima and sums
+  float* part_o = reinterpret_cast<float*>(ring);
+  float* part_m = part_o + 2 * kWtRows * D;
+  float* part_l = part_m + 2 * kWtRows;
+  static_assert(2 * kWtRows * (D + 2) * 4 <= kStages * S::kTile, "the ring holds a split's result");
 
   if (warp >= 8) {
     if (row0 >= rows) {
@@ -373,10 +389,14 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         return ok;
       };
       int nk = 0, nv = 0;  // tiles asked for
-      for (; nv < min(n, kSV); ++nv) {
-        const int row = box_row(nv);
-        if (nv < kSK) load(tm_k, nk++, row);
-        load(tm_v, kSK + nv, row);
+      constexpr int kFirst = kSK > kSV ? kSK : kSV;
+      int rows_of[kFirst];  // the look-ups of the first tiles run side by side
+#pragma unroll
+      for (int j = 0; j < kFirst; ++j) rows_of[j] = j < n ? box_row(j) : none;
+#pragma unroll
+      for (int j = 0; j < kFirst; ++j) {
+        if (j < min(n, kSK)) load(tm_k, nk++, rows_of[j]);
+        if (j < min(n, kSV)) load(tm_v, kSK + nv++, rows_of[j]);
       }
       bool ok = n == 0 || look_over(0);
       for (int j = 0; j < n && ok; ++j) {
@@ -516,10 +536,17 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       const float sl2 = a.scale_log2;
       // whether some page in sight is not there: only then are the tiles' pages looked up
       bool hole = false;
-      for (int j = 0; j < 2; ++j) {
-        const int p0 = j ? mine.lo.start / a.page_tokens : 0;
-        const int p1 = ((j ? mine.hi.end : mine.hi.sink_end) + a.page_tokens - 1) / a.page_tokens;
-        for (int x = p0 + lane; x < p1; x += 32) hole = hole || table[x] < 0 || table[x] >= a.pages;
+      if (n > 0) {
+        const int last_sink = min(n, max(tiles.sink, 0));  // sink tiles of this CTA, then window tiles
+        for (int j = 0; j < 2; ++j) {
+          const int t0 = j ? last_sink : 0, t1 = j ? n : last_sink;
+          if (t0 == t1) continue;
+          const int p0 = tiles.tile(t0) * kWtKeys / a.page_tokens;
+          const int p1 = min((min((tiles.tile(t1 - 1) + 1) * kWtKeys, mine.hi.end) + a.page_tokens - 1) / a.page_tokens,
+                             a.width);
+#pragma unroll 4
+          for (int x = p0 + lane; x < p1; x += 32) hole |= static_cast<uint32_t>(table[x]) >= static_cast<uint32_t>(a.pages);
+        }
       }
       const bool holes = __any_sync(0xffffffffu, hole && mine.any);
       float m = -INFINITY, l = 0.0f;
@@ -629,8 +656,26 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       if (ok && np > 0) ok = mbar_wait(&pv_done[i], (np - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
+      if (splits > 1) {
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // both tiles' MMAs have read the ring
+        const int rr = i * kWtRows + r;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32] = {};
+          if (np > 0) {
+            tmem_ld32_nowait(o_addr + c * 32, o);
+            tmem_wait_ld(o);
+          }
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            *reinterpret_cast<uint4*>(part_o + rr * D + (((c * 8 + x) ^ (rr & 7)) << 2)) =
+                make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+        }
+        part_m[rr] = ok ? m : __uint_as_float(0x7fffffffu);
+        part_l[rr] = l;
+      }
       // warp 9's mark: every tile it looked at was multiplied before pv_done
-      if (ok && *reinterpret_cast<volatile uint32_t*>(dirty)) {
+      else if (ok && *reinterpret_cast<volatile uint32_t*>(dirty)) {
         for (int x = 0; x < 32; ++x) {
           const int rr = row0 + i * kWtRows + quarter * 32 + x;
           if (rr < row1) window_row<T, D>(a, b, seq, rr / a.group, kvh * a.group + rr % a.group, lane);
@@ -678,9 +723,57 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       }
     }
     // more rows than the launch was told of: one by one
-    if (tile_id == row_tiles - 1)
+    if (tile_id == row_tiles - 1 && rank == 0)
       for (int r = row_tiles * (2 * kWtRows) + warp; r < rows; r += 8)
         window_row<T, D>(a, b, seq, r / a.group, kvh * a.group + r % a.group, lane);
+  }
+  if (splits > 1) {
+    // join the cluster's results in rank order, each CTA a share of the rows
+    cluster_sync_all();
+    if (warp < 8 && row0 < rows) {
+      uint32_t marked = 0;
+      for (int x = 0; x < splits; ++x) marked |= __float_as_uint(ld_cluster(mapa_shared(smem_u32(dirty), x)));
+      if (marked) {
+        for (int r = row0 + rank * 8 + warp; r < row1; r += splits * 8)
+          window_row<T, D>(a, b, seq, r / a.group, kvh * a.group + r % a.group, lane);
+      } else {
+        const float sl2 = a.scale_log2;
+        for (int e = rank * 256 + threadIdx.x; e < (row1 - row0) * (D / 8); e += splits * 256) {
+          const int r = e / (D / 8), ch = e % (D / 8) * 2;
+          float mx[kWinSplits], top = -INFINITY;  // all loads in flight at once
+#pragma unroll
+          for (int x = 0; x < kWinSplits; ++x) {
+            mx[x] = -INFINITY;
+            if (x < splits) mx[x] = ld_cluster(mapa_shared(smem_u32(part_m + r), x));
+          }
+#pragma unroll
+          for (int x = 0; x < kWinSplits; ++x) top = max3_nan(top, mx[x], mx[x]);
+          float sum = 0.0f;
+          float4 u = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = u;
+#pragma unroll
+          for (int x = 0; x < kWinSplits; ++x) {
+            if (x >= splits) continue;
+            const float f = mx[x] == -INFINITY ? 0.0f : ex2((mx[x] - top) * sl2);
+            const float4 p = ld_cluster4(mapa_shared(smem_u32(part_o + r * D + ((ch ^ (r & 7)) << 2)), x));
+            const float4 q = ld_cluster4(mapa_shared(smem_u32(part_o + r * D + (((ch + 1) ^ (r & 7)) << 2)), x));
+            sum += f * ld_cluster(mapa_shared(smem_u32(part_l + r), x));
+            u.x = fmaf(f, p.x, u.x), u.y = fmaf(f, p.y, u.y), u.z = fmaf(f, p.z, u.z), u.w = fmaf(f, p.w, u.w);
+            v.x = fmaf(f, q.x, v.x), v.y = fmaf(f, q.y, v.y), v.z = fmaf(f, q.z, v.z), v.w = fmaf(f, q.w, v.w);
+          }
+          const bool none = sum == 0.0f;
+          const float inv = none ? 0.0f : 1.0f / sum;
+          uint4 w4 = make_uint4(pack2<T>(u.x * inv, u.y * inv), pack2<T>(u.z * inv, u.w * inv),
+                                pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+          if (none) w4 = make_uint4(0, 0, 0, 0);
+          const int qr = row0 + r, head = kvh * a.group + qr % a.group;
+          const long long tok = seq.q0 + qr / a.group;
+          *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs + ch * 4) = w4;
+          if (a.lse && ch == 0)
+            a.lse[tok * a.heads + head] = none ? -INFINITY : (top * sl2 + log2f(sum)) * 0.6931471805599453f;
+        }
+      }
+    }
+    cluster_sync_all();  // the others have read this CTA's part
   }
   tc_fence_before();
   __syncthreads();
