@@ -11,6 +11,23 @@
 
 namespace oasis {
 
+// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery, "Division by invariant
+// integers using multiplication", 1994): the integer divisions of a dozen rows are otherwise a
+// microsecond before the first load.
+struct FastDiv {
+  int d;
+  uint32_t mul, shift;
+  __device__ __forceinline__ int div(int n) const {
+    return static_cast<int>((__umulhi(mul, static_cast<uint32_t>(n)) + static_cast<uint32_t>(n)) >> shift);
+  }
+  __device__ __forceinline__ int mod(int n) const { return n - div(n) * d; }
+};
+inline FastDiv fast_div(int d) {
+  uint32_t shift = 0;
+  while ((1ull << shift) < static_cast<uint64_t>(d)) ++shift;
+  return {d, static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1), shift};
+}
+
 struct WinArgs {
   const void* q;
   void* out;
@@ -18,6 +35,7 @@ struct WinArgs {
   long long q_ts, q_hs, o_ts, o_hs;
   const void *k, *v;
   int pages, kv_heads, page_tokens;
+  FastDiv by_page, by_group, by_frame;
   const int32_t* table;
   int width;
   const int32_t *kv_len, *cu_q;
@@ -52,7 +70,7 @@ struct WinRange {
 __device__ __forceinline__ WinRange win_range(const WinArgs& a, int pos, int kv) {
   WinRange r = {0, 0, 0};
   if (pos < 0) return r;  // more queries than cached tokens
-  const int f = pos / a.frame;
+  const int f = a.by_frame.div(pos);
   r.end = static_cast<int>(min(static_cast<long long>(f + 1) * a.frame, static_cast<long long>(kv)));
   if (a.window && f >= a.window) {
     r.start = (f - a.window + 1) * a.frame;
@@ -96,7 +114,7 @@ __device__ __noinline__ void window_row(const WinArgs& a, int b, const WinSeq& s
   const long long row = s.q0 + qi;
   const T* q = static_cast<const T*>(a.q) + row * a.q_ts + head * a.q_hs + lane * E;
   const WinRange r = win_range(a, s.kv - s.n_q + qi, s.kv);
-  const int kvh = head / a.group;
+  const int kvh = a.by_group.div(head);
   const int32_t* table = a.table + static_cast<long long>(b) * a.width;
   float qv[E], o[E];
 #pragma unroll
@@ -110,10 +128,10 @@ __device__ __noinline__ void window_row(const WinArgs& a, int b, const WinSeq& s
     const int hi = part ? r.end : r.sink_end;
 #pragma unroll 1
     for (int key = part ? r.start : 0; key < hi; ++key) {
-      const int page = table[key / a.page_tokens];
+      const int page = table[a.by_page.div(key)];
       if (page < 0 || page >= a.pages) continue;
       const long long off =
-          ((static_cast<long long>(page) * a.kv_heads + kvh) * a.page_tokens + key % a.page_tokens) * D + lane * E;
+          ((static_cast<long long>(page) * a.kv_heads + kvh) * a.page_tokens + a.by_page.mod(key)) * D + lane * E;
       const T* k = static_cast<const T*>(a.k) + off;
       const T* v = static_cast<const T*>(a.v) + off;
       float d = 0.0f;
@@ -181,18 +199,47 @@ inline long long visible_keys(const WinArgs& a, int max_kv) {
   return std::min<long long>(max_kv, (static_cast<long long>(a.window) + a.sinks) * a.frame);
 }
 
+// Clusters of `size` CTAs of a tile kernel that fit the device at once (a cluster lies within a GPC),
+// asked once per device; 0 where the question fails.
+template <typename T, int D>
+int tile_clusters(int size) {
+  static std::atomic<int> known[64][kWinSplits];  // + 1
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev < 64)
+    if (const int k = known[dev][size - 1].load(std::memory_order_relaxed)) return k - 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size);
+  cfg.blockDim = dim3(kWtThreads);
+  cfg.dynamicSmemBytes = WtShape<D>::kSmem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, attn_window_tile_kernel<T, D>, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    n = 0;
+  }
+  if (dev < 64) known[dev][size - 1].store(n + 1, std::memory_order_relaxed);
+  return n;
+}
+
 // CTAs of a cluster that share the keys of one pair of query tiles: the count of least estimated
-// time, where a CTA costs its key tiles and about 3 more to begin and end, joining 2 more, and
-// a wave is one CTA per SM (clusters of 8 fill 128 SMs: they lie within a GPC).
-inline int tile_splits(long long pairs, long long keys) {
+// time, where a CTA costs its key tiles and about 3 more to begin and end, joining 2 more.
+template <typename T, int D>
+int tile_splits(long long pairs, long long keys) {
   const long long tiles = (keys + kWtKeys - 1) / kWtKeys;
   int best = 1;
   double least = 0.0;
-  for (int s = 1; s <= kWinSplits; s *= 2) {
-    const long long sms = s == 8 ? 128 : num_sms() / s * s;
-    const double cost = static_cast<double>((pairs * s + sms - 1) / sms) *
+  for (int s = 1; s <= kWinSplits; ++s) {
+    const long long fit = tile_clusters<T, D>(s);
+    if (fit <= 0) continue;
+    const double cost = static_cast<double>((pairs + fit - 1) / fit) *
                         (static_cast<double>((tiles + s - 1) / s) + 3.0 + (s > 1 ? 2.0 : 0.0));
-    if (s == 1 || cost < least) {
+    if (least == 0.0 || cost < least) {
       best = s;
       least = cost;
     }
@@ -223,7 +270,7 @@ int launch_attn_window(const WinArgs& a, int max_q, int max_kv, cudaStream_t str
     if (int st = encode_page_rows(&tv, a.v, a, D, box)) return st;
     if (int st = allow_smem<attn_window_tile_kernel<T, D>>(WtShape<D>::kSmem, "attn_window_tile_kernel")) return st;
     const int row_tiles = static_cast<int>((max_rows + 2 * kWtRows - 1) / (2 * kWtRows));
-    const int splits = tile_splits(static_cast<long long>(row_tiles) * a.kv_heads * a.batch, visible_keys(a, max_kv));
+    const int splits = tile_splits<T, D>(static_cast<long long>(row_tiles) * a.kv_heads * a.batch, visible_keys(a, max_kv));
     if (static_cast<long long>(row_tiles) * a.kv_heads * splits > 0x7fffffffLL)
       return fail(OASIS_ERR_UNSUPPORTED, "oasis_attn_window: too many query rows");
     cudaError_t e = launch_pdl_cluster(attn_window_tile_kernel<T, D>, dim3(row_tiles * a.kv_heads * splits, 1, a.batch),
@@ -261,6 +308,8 @@ extern "C" int oasis_attn_window(const oasis_attn_window_t* p, cudaStream_t stre
     return fail(OASIS_ERR_UNSUPPORTED, std::string(who) + ": at most 65535 sequences and heads");
   if (static_cast<long long>(p->table_width) * p->page_tokens > 0x3fffffffLL)
     return fail(OASIS_ERR_UNSUPPORTED, std::string(who) + ": at most 2^30 - 1 tokens per sequence");
+  if (static_cast<long long>(p->tokens) * (p->heads / p->kv_heads) > 0x7fffff00LL)
+    return fail(OASIS_ERR_UNSUPPORTED, std::string(who) + ": more than 2^31 query rows per key head");
   if (!p->cu_q && p->tokens != p->batch)
     return fail(OASIS_ERR_INVALID_ARG, std::string(who) + ": without cu_q there is one query per sequence");
   if (p->batch == 0 || p->tokens == 0) return OASIS_OK;
@@ -286,6 +335,7 @@ extern "C" int oasis_attn_window(const oasis_attn_window_t* p, cudaStream_t stre
   a.frame = std::min(p->frame_tokens, 0x3fffffff);
   a.window = p->window;
   a.sinks = p->sinks;
+  a.by_page = fast_div(a.page_tokens), a.by_group = fast_div(a.group), a.by_frame = fast_div(a.frame);
   a.scale_log2 = p->scale * 1.4426950408889634f;
   const int capacity = p->table_width * p->page_tokens;
   const int max_q = !p->cu_q ? 1 : p->max_q > 0 ? std::min(p->max_q, p->tokens) : p->tokens;

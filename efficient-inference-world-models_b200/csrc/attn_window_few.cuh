@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, D == 64 ? (NR == 8 ? 4 : 3) : 
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const int r = row0 + g + 8 * t;
-      range[t] = r < row1 ? win_range(a, seq.kv - seq.n_q + r / a.group, seq.kv) : WinRange{0, 0, 0};
+      range[t] = r < row1 ? win_range(a, seq.kv - seq.n_q + a.by_group.div(r), seq.kv) : WinRange{0, 0, 0};
     }
     uint4 q[RT][KC];
 #pragma unroll
@@ -90,8 +90,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, D == 64 ? (NR == 8 ? 4 : 3) : 
         q[t][i] = make_uint4(0, 0, 0, 0);
         if (r < row1)
           q[t][i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
-                                                    static_cast<long long>(seq.q0 + r / a.group) * a.q_ts +
-                                                    (kvh * a.group + r % a.group) * a.q_hs + (4 * i + c) * 8);
+                                                    static_cast<long long>(seq.q0 + a.by_group.div(r)) * a.q_ts +
+                                                    (kvh * a.group + a.by_group.mod(r)) * a.q_hs + (4 * i + c) * 8);
       }
     }
     float o[VC][4][RT][4];
@@ -117,11 +117,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, D == 64 ? (NR == 8 ? 4 : 3) : 
     const int j1 = static_cast<int>(static_cast<long long>(steps.n) * (part + 1) / parts);
     uint4 kb[2][KC], vb[4][VC];
     auto look_up = [&](int j) {  // page of a step, -1: none
-      const int idx = j < j1 ? steps.tile(j) * 16 / a.page_tokens : a.width;
+      const int idx = j < j1 ? a.by_page.div(steps.tile(j) * 16) : a.width;
       return idx < a.width ? table[idx] : -1;
     };
     auto base_of = [&](int j, int page) {  // first element of the step's first key
-      const int at = steps.tile(j) * 16 % a.page_tokens;
+      const int at = a.by_page.mod(steps.tile(j) * 16);
       return ((static_cast<long long>(page) * a.kv_heads + kvh) * a.page_tokens + at) * D;
     };
     auto there = [&](int page) { return page >= 0 && page < a.pages; };
@@ -316,9 +316,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, D == 64 ? (NR == 8 ? 4 : 3) : 
       if (x < splits) marked |= __float_as_uint(ld_cluster(mapa_shared(smem_u32(&sh.dirty), x)));
     if (marked) {
       for (int r = row0 + part; r < row1; r += parts)
-        window_row<T, D>(a, b, seq, r / a.group, kvh * a.group + r % a.group, lane);
+        window_row<T, D>(a, b, seq, a.by_group.div(r), kvh * a.group + a.by_group.mod(r), lane);
     } else {
-      for (int e = split * kFewWarps * 32 + threadIdx.x; e < (row1 - row0) * (D / 4); e += splits * kFewWarps * 32) {
+      for (int e = threadIdx.x * splits + split; e < (row1 - row0) * (D / 4); e += splits * kFewWarps * 32) {
         const int r = e / (D / 4), d = (e % (D / 4)) * 4;
         float mx[kWinSplits], top = -INFINITY;  // all loads in flight at once
 #pragma unroll
@@ -341,8 +341,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, D == 64 ? (NR == 8 ? 4 : 3) : 
         }
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const int qr = row0 + r;
-        const long long tok = seq.q0 + qr / a.group;
-        const int head = kvh * a.group + qr % a.group;
+        const long long tok = seq.q0 + a.by_group.div(qr);
+        const int head = kvh * a.group + a.by_group.mod(qr);
         const bool none = sum == 0.0f;
         uint2 w2 = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
         if (none) w2 = make_uint2(0, 0);

@@ -232,9 +232,9 @@ struct WtSpan {
 __device__ __forceinline__ WtSpan wt_span(const WinArgs& a, const WinSeq& s, int row0, int row1) {
   WtSpan w;
   const int base = s.kv - s.n_q;
-  const int p1 = base + (row1 - 1) / a.group;
+  const int p1 = base + a.by_group.div(max(row1 - 1, 0));
   w.any = row0 < row1 && p1 >= 0;
-  w.lo = win_range(a, base + row0 / a.group, s.kv);  // all zero where the position is negative
+  w.lo = win_range(a, base + a.by_group.div(row0), s.kv);  // all zero where the position is negative
   w.hi = win_range(a, p1, s.kv);
   return w;
 }
@@ -340,15 +340,14 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       // rows that no query of this CTA sees (ends of pages, tokens before the window) are zeroed, since
       // their weights are 0 but 0 * NaN is not; an infinity or NaN in a row that only some queries
       // see marks the CTA, whose rows are then computed one by one (window_row).
-      const int boxes = kWtKeys / box_rows, page_boxes = a.page_tokens / box_rows;
+      const int boxes = kWtKeys / box_rows;
       const int none = a.pages * a.kv_heads * a.page_tokens;  // beyond the pages: zeros
       auto box_row = [&](int j) {  // lane x takes box x
-        const int box = tiles.tile(j) * boxes + lane;
-        const int idx = box / page_boxes;
+        const int key = tiles.tile(j) * kWtKeys + lane * box_rows;
+        const int idx = a.by_page.div(key);
         const int page = idx < a.width ? table[idx] : -1;
-        return page >= 0 && page < a.pages
-                   ? (page * a.kv_heads + kvh) * a.page_tokens + (box - idx * page_boxes) * box_rows
-                   : none;
+        return page >= 0 && page < a.pages ? (page * a.kv_heads + kvh) * a.page_tokens + (key - idx * a.page_tokens)
+                                           : none;
       };
       auto load = [&](const CUtensorMap& map, int slot, int row) {
         if (lane == 0) mbar_arrive_expect_tx(&full[slot], S::kTile);
@@ -519,8 +518,8 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         const int qrow = row0 + i * kWtRows + rr;
         uint4 val = make_uint4(0, 0, 0, 0);
         if (qrow < row1) {
-          const T* src = static_cast<const T*>(a.q) + static_cast<long long>(seq.q0 + qrow / a.group) * a.q_ts +
-                         (kvh * a.group + qrow % a.group) * a.q_hs + ch * 8;
+          const T* src = static_cast<const T*>(a.q) + static_cast<long long>(seq.q0 + a.by_group.div(qrow)) * a.q_ts +
+                         (kvh * a.group + a.by_group.mod(qrow)) * a.q_hs + ch * 8;
           val = *reinterpret_cast<const uint4*>(src);
         }
         *reinterpret_cast<uint4*>(q_tile + (ch >> 3) * S::kHalf + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = val;
@@ -530,7 +529,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       if (lane == 0) mbar_arrive(q_full);
 
       const WinRange range =
-          row < row1 ? win_range(a, seq.kv - seq.n_q + row / a.group, seq.kv) : WinRange{0, 0, 0};
+          row < row1 ? win_range(a, seq.kv - seq.n_q + a.by_group.div(row), seq.kv) : WinRange{0, 0, 0};
       const uint32_t s_addr = tmem + i * 128 + (static_cast<uint32_t>(quarter * 32) << 16);
       const uint32_t o_addr = tmem + 256 + i * D + (static_cast<uint32_t>(quarter * 32) << 16);
       const float sl2 = a.scale_log2;
@@ -541,9 +540,8 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         for (int j = 0; j < 2; ++j) {
           const int t0 = j ? last_sink : 0, t1 = j ? n : last_sink;
           if (t0 == t1) continue;
-          const int p0 = tiles.tile(t0) * kWtKeys / a.page_tokens;
-          const int p1 = min((min((tiles.tile(t1 - 1) + 1) * kWtKeys, mine.hi.end) + a.page_tokens - 1) / a.page_tokens,
-                             a.width);
+          const int p0 = a.by_page.div(tiles.tile(t0) * kWtKeys);
+          const int p1 = min(a.by_page.div(min((tiles.tile(t1 - 1) + 1) * kWtKeys, mine.hi.end) + a.page_tokens - 1), a.width);
 #pragma unroll 4
           for (int x = p0 + lane; x < p1; x += 32) hole |= static_cast<uint32_t>(table[x]) >= static_cast<uint32_t>(a.pages);
         }
@@ -572,7 +570,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
             if (holes) {
 #pragma unroll
               for (int x = 0; x < 32; x += 16) {  // a page is a multiple of 16 tokens
-                const int idx = (k + x) / a.page_tokens;
+                const int idx = a.by_page.div(k + x);
                 const int page = idx < a.width ? table[idx] : -1;
                 if (page < 0 || page >= a.pages) seen &= ~(0xffffu << x);
               }
@@ -678,7 +676,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       else if (ok && *reinterpret_cast<volatile uint32_t*>(dirty)) {
         for (int x = 0; x < 32; ++x) {
           const int rr = row0 + i * kWtRows + quarter * 32 + x;
-          if (rr < row1) window_row<T, D>(a, b, seq, rr / a.group, kvh * a.group + rr % a.group, lane);
+          if (rr < row1) window_row<T, D>(a, b, seq, a.by_group.div(rr), kvh * a.group + a.by_group.mod(rr), lane);
         }
       } else if (ok) {
         // O / l through the warp's own rows of the Q tile (its last reader is done), then out in
@@ -711,21 +709,21 @@ __global__ void __launch_bounds__(kWtThreads, 1)
           const int rr = quarter * 32 + c / kChunks, ch = c % kChunks;
           const int orow = row0 + i * kWtRows + rr;
           if (orow < row1) {
-            T* dst = static_cast<T*>(a.out) + static_cast<long long>(seq.q0 + orow / a.group) * a.o_ts +
-                     (kvh * a.group + orow % a.group) * a.o_hs + ch * 8;
+            T* dst = static_cast<T*>(a.out) + static_cast<long long>(seq.q0 + a.by_group.div(orow)) * a.o_ts +
+                     (kvh * a.group + a.by_group.mod(orow)) * a.o_hs + ch * 8;
             *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(
                 q_tile + (ch >> 3) * S::kHalf + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4));
           }
         }
         if (a.lse && row < row1)
-          a.lse[static_cast<long long>(seq.q0 + row / a.group) * a.heads + kvh * a.group + row % a.group] =
+          a.lse[static_cast<long long>(seq.q0 + a.by_group.div(row)) * a.heads + kvh * a.group + a.by_group.mod(row)] =
               l == 0.0f ? -INFINITY : (m * sl2 + log2f(l)) * 0.6931471805599453f;
       }
     }
     // more rows than the launch was told of: one by one
     if (tile_id == row_tiles - 1 && rank == 0)
       for (int r = row_tiles * (2 * kWtRows) + warp; r < rows; r += 8)
-        window_row<T, D>(a, b, seq, r / a.group, kvh * a.group + r % a.group, lane);
+        window_row<T, D>(a, b, seq, a.by_group.div(r), kvh * a.group + a.by_group.mod(r), lane);
   }
   if (splits > 1) {
     // join the cluster's results in rank order, each CTA a share of the rows
@@ -735,10 +733,10 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       for (int x = 0; x < splits; ++x) marked |= __float_as_uint(ld_cluster(mapa_shared(smem_u32(dirty), x)));
       if (marked) {
         for (int r = row0 + rank * 8 + warp; r < row1; r += splits * 8)
-          window_row<T, D>(a, b, seq, r / a.group, kvh * a.group + r % a.group, lane);
+          window_row<T, D>(a, b, seq, a.by_group.div(r), kvh * a.group + a.by_group.mod(r), lane);
       } else {
         const float sl2 = a.scale_log2;
-        for (int e = rank * 256 + threadIdx.x; e < (row1 - row0) * (D / 8); e += splits * 256) {
+        for (int e = threadIdx.x * splits + rank; e < (row1 - row0) * (D / 8); e += splits * 256) {
           const int r = e / (D / 8), ch = e % (D / 8) * 2;
           float mx[kWinSplits], top = -INFINITY;  // all loads in flight at once
 #pragma unroll
@@ -765,8 +763,8 @@ __global__ void __launch_bounds__(kWtThreads, 1)
           uint4 w4 = make_uint4(pack2<T>(u.x * inv, u.y * inv), pack2<T>(u.z * inv, u.w * inv),
                                 pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
           if (none) w4 = make_uint4(0, 0, 0, 0);
-          const int qr = row0 + r, head = kvh * a.group + qr % a.group;
-          const long long tok = seq.q0 + qr / a.group;
+          const int qr = row0 + r, head = kvh * a.group + a.by_group.mod(qr);
+          const long long tok = seq.q0 + a.by_group.div(qr);
           *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs + ch * 4) = w4;
           if (a.lse && ch == 0)
             a.lse[tok * a.heads + head] = none ? -INFINITY : (top * sl2 + log2f(sum)) * 0.6931471805599453f;
