@@ -10,7 +10,8 @@
 // For tile i and key tile j:  S_i = Q_i K_j^T (TMEM, 128 columns), the softmax thread takes
 // P = exp2(S * scale - m) and writes it in 16 bits over S, O_i += P_i V_j (P from TMEM).  The MMA warp
 // alternates PV_0(j), QK_0(j+1), PV_1(j), QK_1(j+1): while one tile's softmax runs, the tensor
-// cores work for the other.  m is the running maximum, moved (and O rescaled) only when it
+// cores work for the other.  At D = 64 there is room for P beside S, and S_i(j+1) is computed while
+// softmax i works on tile j.  m is the running maximum, moved (and O rescaled) only when it
 // grows by more than 2^8, which keeps every p below 2^8 and the sum exact to fp32.
 #pragma once
 
@@ -19,7 +20,6 @@ namespace oasis {
 constexpr int kWtRows = 128;     // query rows of a tile
 constexpr int kWtKeys = 128;     // keys of a K/V tile
 constexpr int kWtThreads = 320;  // 8 softmax warps, MMA, loads: 200 registers each
-constexpr int kWtPolyEvery = 3;  // of the weights' pairs, one in three is computed without the SFU
 constexpr float kWtLazy = 8.0f;  // log2 of how far scores may pass the maximum in use
 
 template <int D>
@@ -29,7 +29,13 @@ struct WtShape {
   // a K tile is done with a step before the V tile of the same keys: fewer of them
   static constexpr int kStagesK = D == 128 ? 2 : 4, kStagesV = D == 128 ? 3 : 4;
   static constexpr int kStages = kStagesK + kStagesV;
-  static constexpr int kBars = 3 * kStages + 10;
+  static constexpr int kBars = 3 * kStages + 12;
+  // D = 64 leaves TMEM columns for P beside S: the next S is then computed under the softmax
+  static constexpr bool kEarly = D == 64;
+  // quarters of P that the MMAs get before the rest is there: 456 us with two against 465 with three
+  // for a prompt of 8,191 tokens at D = 128, 75 against 71 us for 8 sessions' frames at D = 64
+  static constexpr int kHandover = kEarly ? 3 : 2;
+  static constexpr int kO = 256, kP = kEarly ? kO + 2 * D : 0, kPStep = kEarly ? 64 : 128;  // columns of tile 0, 1
   static constexpr int kSmem = (2 + kStages) * kTile + 1024 + 256 + 8 * kBars;
 };
 
@@ -96,19 +102,15 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
                : "memory");
   asm volatile("" : "+r"(r[30]), "+r"(r[31])::"memory");
 }
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
+// Waits for the stores so far, after `r` has been computed.
+__device__ __forceinline__ void tmem_wait_st(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::st.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15])
+               :
+               : "memory");
 }
-
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -148,27 +150,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float d;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
-}
-
-// 2^x of two fp32 on the multiply-add pipes: x = n + f with n the nearest integer (read off the
-// low bits of x + 1.5 2^23), 2^f by the minimax polynomial of degree 5 on [-1/2, 1/2] (found by
-// Remez exchange; relative error 2^-22 with fp32 rounding), n added to the exponent.  x is
-// kept above -126; not for NaN or infinities.
-__device__ __forceinline__ float2 exp2_poly(uint64_t x2) {
-  float2 x = unpair_f32(x2);
-  x2 = pair_f32(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
-  const uint64_t magic = pair_f32(12582912.0f, 12582912.0f), unmagic = pair_f32(-12582912.0f, -12582912.0f);
-  const uint64_t r = add_f32x2(x2, magic);
-  const uint64_t f = fma_f32x2(add_f32x2(r, unmagic), pair_f32(-1.0f, -1.0f), x2);
-  uint64_t p = pair_f32(0.0013276472454890609f, 0.0013276472454890609f);
-  p = fma_f32x2(p, f, pair_f32(0.009675540961325169f, 0.009675540961325169f));
-  p = fma_f32x2(p, f, pair_f32(0.05550713092088699f, 0.05550713092088699f));
-  p = fma_f32x2(p, f, pair_f32(0.24022120237350464f, 0.24022120237350464f));
-  p = fma_f32x2(p, f, pair_f32(0.6931469440460205f, 0.6931469440460205f));
-  p = fma_f32x2(p, f, pair_f32(1.0000001192092896f, 1.0000001192092896f));
-  const float2 e = unpair_f32(p), n = unpair_f32(r);
-  return make_float2(__uint_as_float(__float_as_uint(e.x) + (__float_as_uint(n.x) << 23)),
-                     __uint_as_float(__float_as_uint(e.y) + (__float_as_uint(n.y) << 23)));
 }
 
 // Bits lo..hi-1 of a word, both clamped to it.
@@ -277,7 +258,8 @@ __global__ void __launch_bounds__(kWtThreads, 1)
   uint64_t* p_full = s_full + 2;   // [2]
   uint64_t* p_half = p_full + 2;   // [2]
   uint64_t* pv_done = p_half + 2;  // [2]
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(pv_done + 2);
+  uint64_t* s_free = pv_done + 2;  // [2] (kEarly)
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(s_free + 2);
   uint32_t* dirty = tmem_holder + 1;
 
   pdl_trigger();
@@ -294,6 +276,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       mbar_init(&p_full[i], 4);
       mbar_init(&p_half[i], 4);
       mbar_init(&pv_done[i], 1);
+      mbar_init(&s_free[i], 4);
     }
     *dirty = 0;
     mbar_fence_init();
@@ -430,12 +413,16 @@ __global__ void __launch_bounds__(kWtThreads, 1)
           umma_ss(tmem + i * 128, qa + (k >> 2) * kHalf16 + (k & 3) * 2, ka + (k >> 2) * kHalf16 + (k & 3) * 2, idesc_s,
                   k > 0);
       };
-      auto pv = [&](int i, int st, int k0, uint32_t acc) {  // half of the keys
+      auto pv = [&](int i, int st, auto first, auto last, uint32_t acc) {  // keys 16 first .. 16 last - 1
         const uint64_t va = v_desc + st * kTile16;
 #pragma unroll
-        for (int k = k0; k < k0 + kWtKeys / 32; ++k)
-          umma_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8, va + k * 128, idesc_o, k == k0 ? acc : 1u);
+        for (int k = decltype(first)::value; k < decltype(last)::value; ++k)
+          umma_ts(tmem + S::kO + i * D, tmem + S::kP + i * S::kPStep + k * 8, va + k * 128, idesc_o,
+                  k == 0 ? acc : 1u);
       };
+      using Zero = std::integral_constant<int, 0>;
+      using Hand = std::integral_constant<int, S::kHandover * 2>;
+      using All = std::integral_constant<int, kWtKeys / 16>;
       bool ok = mbar_wait(q_full, 0);
       uint32_t np0 = 0, np1 = 0;  // P tiles taken
       if (n > 0) {
@@ -455,49 +442,91 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         }
         __syncwarp();
       }
-      // PV_i(j), then QK_i(j+1)
-      auto turn = [&](int i, uint32_t& np, bool now, bool next, int vs, int ks) {
-        if (now) {
-          ok = __all_sync(0xffffffffu, ok && mbar_wait(&p_half[i], np & 1));
-          if (!ok) return;
-          tc_fence_after();
-          if (elect_one()) pv(i, vs, 0, np > 0);
-          __syncwarp();
-          ok = __all_sync(0xffffffffu, mbar_wait(&p_full[i], np & 1));
-          if (!ok) return;
-          tc_fence_after();
-          if (elect_one()) {
-            pv(i, vs, kWtKeys / 32, 1u);
-            umma_commit(&pv_done[i]);
-          }
-          __syncwarp();
-          ++np;
-        }
-        if (next) {
-          if (elect_one()) {
-            qk(i, ks);
-            umma_commit(&s_full[i]);
-          }
-          __syncwarp();
-        }
-      };
-      for (int j = 0; j < n && ok; ++j) {
-        const int k0 = tiles.tile(j) * kWtKeys, k1 = j + 1 < n ? tiles.tile(j + 1) * kWtKeys : 0;
-        const bool more = j + 1 < n;
-        const int vs = kSK + j % kSV, ks = (j + 1) % kSK;
-        ok = mbar_wait(&full[vs], (j / kSV) & 1) && mbar_wait(&clean[vs], (j / kSV) & 1);
-        if (ok && more) ok = mbar_wait(&full[ks], ((j + 1) / kSK) & 1);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+      // PV_i in two pieces, the second when the rest of P is there
+      auto multiply = [&](int i, uint32_t& np, int vs) {
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(&p_half[i], np & 1));
+        if (!ok) return;
         tc_fence_after();
-        turn(0, np0, half[0].some(k0, k0 + kWtKeys), more && half[0].some(k1, k1 + kWtKeys), vs, ks);
-        turn(1, np1, half[1].some(k0, k0 + kWtKeys), more && half[1].some(k1, k1 + kWtKeys), vs, ks);
-        if (!ok) break;
+        if (elect_one()) pv(i, vs, Zero{}, Hand{}, np > 0);
+        __syncwarp();
+        ok = __all_sync(0xffffffffu, mbar_wait(&p_full[i], np & 1));
+        if (!ok) return;
+        tc_fence_after();
         if (elect_one()) {
-          umma_commit(&empty[vs]);
-          if (more) umma_commit(&empty[ks]);
+          pv(i, vs, Hand{}, All{}, 1u);
+          umma_commit(&pv_done[i]);
         }
         __syncwarp();
+        ++np;
+      };
+      auto score = [&](int i, int ks) {
+        if (elect_one()) {
+          qk(i, ks);
+          umma_commit(&s_full[i]);
+        }
+        __syncwarp();
+      };
+      auto release = [&](int slot) {
+        if (elect_one()) umma_commit(&empty[slot]);
+        __syncwarp();
+      };
+      auto seen = [&](int i, int j) {
+        const int k0 = tiles.tile(j) * kWtKeys;
+        return (i ? half[1] : half[0]).some(k0, k0 + kWtKeys);
+      };
+      if (S::kEarly) {
+        // QK_0(j+1), PV_1(j-1), QK_1(j+1), PV_0(j): S of the next tile as soon as the softmax has
+        // this one in registers
+        uint32_t ns0 = n > 0 && seen(0, 0), ns1 = n > 0 && seen(1, 0);  // S tiles issued
+        auto next_score = [&](int i, uint32_t& ns, int j) {
+          if (!seen(i, j)) return;
+          if (ns > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(&s_free[i], (ns - 1) & 1));
+          if (!ok) return;
+          tc_fence_after();
+          score(i, j % kSK);
+          ++ns;
+        };
+        for (int j = 0; j <= n && ok; ++j) {
+          const bool more = j + 1 < n;
+          if (more) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&full[(j + 1) % kSK], ((j + 1) / kSK) & 1));
+            if (ok) next_score(0, ns0, j + 1);
+          }
+          if (ok && j > 0) {
+            const int vs = kSK + (j - 1) % kSV;
+            if (seen(1, j - 1)) multiply(1, np1, vs);
+            if (ok) release(vs);
+          }
+          if (ok && more) {
+            next_score(1, ns1, j + 1);
+            if (ok) release((j + 1) % kSK);
+          }
+          if (ok && j < n) {
+            const int vs = kSK + j % kSV;
+            ok = mbar_wait(&full[vs], (j / kSV) & 1) && mbar_wait(&clean[vs], (j / kSV) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+            if (ok && seen(0, j)) multiply(0, np0, vs);
+          }
+        }
+      } else {
+        // PV_0(j), QK_0(j+1), PV_1(j), QK_1(j+1)
+        for (int j = 0; j < n && ok; ++j) {
+          const bool more = j + 1 < n;
+          const int vs = kSK + j % kSV, ks = (j + 1) % kSK;
+          ok = mbar_wait(&full[vs], (j / kSV) & 1) && mbar_wait(&clean[vs], (j / kSV) & 1);
+          if (ok && more) ok = mbar_wait(&full[ks], ((j + 1) / kSK) & 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          if (seen(0, j)) multiply(0, np0, vs);
+          if (ok && more && seen(0, j + 1)) score(0, ks);
+          if (ok && seen(1, j)) multiply(1, np1, vs);
+          if (ok && more && seen(1, j + 1)) score(1, ks);
+          if (!ok) break;
+          release(vs);
+          if (more) release(ks);
+        }
       }
     }
   } else {
@@ -531,7 +560,8 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       const WinRange range =
           row < row1 ? win_range(a, seq.kv - seq.n_q + a.by_group.div(row), seq.kv) : WinRange{0, 0, 0};
       const uint32_t s_addr = tmem + i * 128 + (static_cast<uint32_t>(quarter * 32) << 16);
-      const uint32_t o_addr = tmem + 256 + i * D + (static_cast<uint32_t>(quarter * 32) << 16);
+      const uint32_t p_addr = tmem + S::kP + i * S::kPStep + (static_cast<uint32_t>(quarter * 32) << 16);
+      const uint32_t o_addr = tmem + S::kO + i * D + (static_cast<uint32_t>(quarter * 32) << 16);
       const float sl2 = a.scale_log2;
       // whether some page in sight is not there: only then are the tiles' pages looked up
       bool hole = false;
@@ -553,18 +583,14 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       for (int j = 0; j < n; ++j) {
         const int tile = tiles.tile(j), k0 = tile * kWtKeys;
         if (!mine.some(k0, k0 + kWtKeys)) continue;
+        const bool part = holes || !mine.all(k0, k0 + kWtKeys);
         ok = mbar_wait(&s_full[i], np & 1);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
-        const bool part = holes || !mine.all(k0, k0 + kWtKeys);
         uint32_t v[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32_nowait(s_addr + c * 32, v[c]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_wait_ld(v[c]);
-        if (part) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto maxima = [&](int c) {
+          if (part) {
             const int k = k0 + c * 32;
             uint32_t seen = wt_bits(range.start - k, range.end - k) | wt_bits(-k, range.sink_end - k);
             if (holes) {
@@ -577,13 +603,27 @@ __global__ void __launch_bounds__(kWtThreads, 1)
             }
             wt_hide(v[c], seen);
           }
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int x = 0; x < 32; x += 2)
             mx[(x >> 1) & 3] = max3_nan(mx[(x >> 1) & 3], __uint_as_float(v[c][x]), __uint_as_float(v[c][x + 1]));
+        };
+        tmem_ld32_nowait(s_addr, v[0]);
+        tmem_ld32_nowait(s_addr + 32, v[1]);
+        tmem_wait_ld(v[0]);
+        tmem_wait_ld(v[1]);
+        tmem_ld32_nowait(s_addr + 64, v[2]);
+        tmem_ld32_nowait(s_addr + 96, v[3]);
+        maxima(0);
+        maxima(1);
+        tmem_wait_ld(v[2]);
+        tmem_wait_ld(v[3]);
+        if (S::kEarly) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[i]);
+        }
+        maxima(2);
+        maxima(3);
         const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
         // a NaN score makes the maximum and with it the whole row NaN; a tile without a visible
         // key (top -inf) changes nothing
@@ -608,44 +648,39 @@ __global__ void __launch_bounds__(kWtThreads, 1)
             tmem_st16(o_addr + c * 16, w);
           }
         }
+        // P of the previous tile has been read: with P in place of S that is so since S came after it
+        if (S::kEarly && np > 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[i], (np - 1) & 1));
+          if (!ok) break;
+          tc_fence_after();
+        }
         const float base = m == -INFINITY ? 0.0f : fmaf(m, 0.0f, -m * sl2);  // NaN for a maximum of +inf
         uint64_t sum[2] = {0, 0};
-        // the columns of P lie over those of S, which are all in registers; the MMAs take the
-        // first half of the keys while the second is computed
-        auto weights = [&](auto partial) {
-          constexpr bool PART = decltype(partial)::value;
+        // (D = 128: the columns of P lie over those of S, which are all in registers.)  The MMAs take
+        // the first kHandover quarters of the keys while the rest is computed.
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pk[16];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
 #pragma unroll
-            for (int x = 0; x < 32; x += 2) {
-              const uint64_t t = fma_f32x2(pair_f32(v[c][x], v[c][x + 1]), pair_f32(sl2, sl2), pair_f32(base, base));
-              float2 e = unpair_f32(t);
-              if (!PART && (x >> 1) % kWtPolyEvery == kWtPolyEvery - 1) {
-                e = exp2_poly(t);
-              } else {
-                e.x = ex2(e.x);
-                e.y = ex2(e.y);
-              }
-              sum[(x >> 1) & 1] = add_f32x2(sum[(x >> 1) & 1], pair_f32(e.x, e.y));
-              pk[x / 2] = pack2<T>(e.x, e.y);
-            }
-            tmem_st16(s_addr + c * 16, pk);
-            if (c == 1) {
-              tmem_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&p_half[i]);
-            }
+          for (int x = 0; x < 32; x += 2) {
+            float2 e =
+                unpair_f32(fma_f32x2(pair_f32(v[c][x], v[c][x + 1]), pair_f32(sl2, sl2), pair_f32(base, base)));
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            sum[(x >> 1) & 1] = add_f32x2(sum[(x >> 1) & 1], pair_f32(e.x, e.y));
+            pk[x / 2] = pack2<T>(e.x, e.y);
           }
-        };
-        if (part)
-          weights(std::true_type{});
-        else
-          weights(std::false_type{});
+          if (c == S::kHandover) {
+            tmem_wait_st(pk);  // of the earlier quarters, under the arithmetic of this one
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_half[i]);
+          }
+          tmem_st16(p_addr + c * 16, pk);
+        }
         const float2 s2 = unpair_f32(add_f32x2(sum[0], sum[1]));
         l += s2.x + s2.y;
-        tmem_wait_st();
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[i]);
