@@ -120,31 +120,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 
-// Pairs of fp32 in one 64-bit register: two multiply-adds or sums per instruction.
-__device__ __forceinline__ uint64_t pair_f32(uint32_t lo, uint32_t hi) {
-  uint64_t p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "r"(lo), "r"(hi));
-  return p;
-}
-__device__ __forceinline__ uint64_t pair_f32(float lo, float hi) {
-  return pair_f32(__float_as_uint(lo), __float_as_uint(hi));
-}
-__device__ __forceinline__ float2 unpair_f32(uint64_t p) {
-  uint32_t lo, hi;
-  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(p));
-  return make_float2(__uint_as_float(lo), __uint_as_float(hi));
-}
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 // The larger of three; NaN if one is.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float d;

@@ -1,65 +1,82 @@
 // RMS norm of query and key heads with the rotation over several position axes, in one pass;
 // optionally the append of keys and values into cache pages.
+#include <algorithm>
+
 #include "launch.cuh"
 
 namespace oasis {
 
-// 8 consecutive elements of a row as fp32, and back with one rounding to nearest even.
+// 8 consecutive elements of a row in registers: as four pairs of fp32, and back with one rounding to
+// nearest even.
 template <typename T>
-struct Vec8;
-template <>
-struct Vec8<__nv_bfloat16> {
-  using raw = uint4;
-  static __device__ __forceinline__ void unpack(const raw& r, float (&x)[8]) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+struct Vec8 {
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const T* p) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ Vec8 of_lane(int lane) const {
+    Vec8 r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = bf16_lo(w[i]);
-      x[2 * i + 1] = bf16_hi(w[i]);
-    }
+    for (int i = 0; i < 4; ++i) r.w[i] = __shfl_sync(0xffffffffu, w[i], lane);
+    return r;
   }
-  static __device__ __forceinline__ raw pack(const float (&x)[8]) {
-    return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
-                      pack_bf16x2(x[6], x[7]));
-  }
+  __device__ __forceinline__ uint64_t pair(int i) const;
+  __device__ __forceinline__ void set(int i, uint64_t p);
 };
 template <>
-struct Vec8<__half> {
-  using raw = uint4;
-  static __device__ __forceinline__ void unpack(const raw& r, float (&x)[8]) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-  }
-  static __device__ __forceinline__ raw pack(const float (&x)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  }
-};
-struct alignas(16) Raw32 {
-  float4 a, b;
-};
+__device__ __forceinline__ uint64_t Vec8<__nv_bfloat16>::pair(int i) const {
+  return pair_f32(w[i] << 16, w[i] & 0xFFFF0000u);
+}
+template <>
+__device__ __forceinline__ void Vec8<__nv_bfloat16>::set(int i, uint64_t p) {
+  const float2 f = unpair_f32(p);
+  w[i] = pack_bf16x2(f.x, f.y);
+}
+template <>
+__device__ __forceinline__ uint64_t Vec8<__half>::pair(int i) const {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+  return pair_f32(f.x, f.y);
+}
+template <>
+__device__ __forceinline__ void Vec8<__half>::set(int i, uint64_t p) {
+  const float2 f = unpair_f32(p);
+  const __half2 h = __floats2half2_rn(f.x, f.y);
+  w[i] = *reinterpret_cast<const uint32_t*>(&h);
+}
 template <>
 struct Vec8<float> {
-  using raw = Raw32;
-  static __device__ __forceinline__ void unpack(const raw& r, float (&x)[8]) {
-    x[0] = r.a.x, x[1] = r.a.y, x[2] = r.a.z, x[3] = r.a.w;
-    x[4] = r.b.x, x[5] = r.b.y, x[6] = r.b.z, x[7] = r.b.w;
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = reinterpret_cast<const float4*>(p)[0];
+    b = reinterpret_cast<const float4*>(p)[1];
   }
-  static __device__ __forceinline__ raw pack(const float (&x)[8]) {
-    Raw32 r;
-    r.a = make_float4(x[0], x[1], x[2], x[3]);
-    r.b = make_float4(x[4], x[5], x[6], x[7]);
+  __device__ __forceinline__ void store(float* p) const {
+    reinterpret_cast<float4*>(p)[0] = a;
+    reinterpret_cast<float4*>(p)[1] = b;
+  }
+  __device__ __forceinline__ Vec8 of_lane(int lane) const {
+    Vec8 r;
+    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], lane);
+    r.a = make_float4(y[0], y[1], y[2], y[3]);
+    r.b = make_float4(y[4], y[5], y[6], y[7]);
     return r;
+  }
+  __device__ __forceinline__ uint64_t pair(int i) const {
+    return i == 0 ? pair_f32(a.x, a.y) : i == 1 ? pair_f32(a.z, a.w) : i == 2 ? pair_f32(b.x, b.y) : pair_f32(b.z, b.w);
+  }
+  __device__ __forceinline__ void set(int i, uint64_t p) {
+    const float2 f = unpair_f32(p);
+    if (i == 0) a.x = f.x, a.y = f.y;
+    if (i == 1) a.z = f.x, a.w = f.y;
+    if (i == 2) b.x = f.x, b.y = f.y;
+    if (i == 3) b.z = f.x, b.w = f.y;
   }
 };
 
@@ -83,31 +100,44 @@ struct RopeArgs {
 constexpr int kRopeWarps = 8;
 
 // A head of D elements is spread over L = D / 8 lanes, 8 consecutive elements (16 or 32 bytes)
-// each, so a warp takes 32 / L heads at a time and a mean of squares is log2(L) shuffles.  A CTA
-// takes 8 / warps_per_token tokens.  It first computes the cos and sin of every rotated pair of
-// its tokens into shared memory, one pair per thread: the angle is position * frequency in turns,
-// reduced to [-1/2, 1/2] in fp64 (an fp32 angle of position 10^6 is off by 0.06 rad), then sincospi
-// in fp32.  Each lane keeps the values of its own pairs in registers for all heads of the token.
-// With the half-split pairing the other element of a pair sits in another lane, rot / 16 away, and
-// comes by shuffle.  Bound by HBM (every byte read and written once).
+// each, so a warp takes 32 / L heads at a time and a mean of squares is log2(L) shuffles.  One or,
+// where tokens are few, several warps take a token.  A warp asks for the first rows, then computes the
+// cos and sin of the token's rotated pairs under those loads, one or more pairs per lane, and hands
+// them round through shared memory: the angle is position * frequency in turns, reduced to
+// [-1/2, 1/2] in fp64 (an fp32 angle of position 10^6 is off by 0.06 rad), then sincospi in fp32.
+// Weight and rotation of a lane's 8 elements become two factors each, kept for all heads of the
+// token:  y = rsqrt(mean) * (A x + B x'),  x' the other element of the pair (the lane's own
+// neighbour, or with the half-split pairing that of the lane rot / 16 away, which comes by shuffle as loaded).
+// Bound by HBM (every byte read and written once).
 template <typename T, int D, bool INTERLEAVED, bool NORM>
-__global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
+__global__ void __launch_bounds__(kRopeWarps * 32, 4) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int L = D / 8;
-  constexpr int HPI = 32 / L;  // heads per warp and iteration
-  constexpr int NA = INTERLEAVED ? 4 : 8;
-  using V = Vec8<T>;
-  using raw = typename V::raw;
+  constexpr int HPI = 32 / L;                // heads per warp and row group
+  constexpr int U = sizeof(T) == 4 ? 2 : 4;  // row groups in flight
   __shared__ float2 s_cs[kRopeWarps][D / 2];
   pdl_trigger();
-  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wpt = a.warps_per_token;
-  const int tpc = kRopeWarps / wpt;  // tokens per CTA
-  const long long tok0 = static_cast<long long>(blockIdx.x) * tpc;
+  const long long t = static_cast<long long>(blockIdx.x) * (kRopeWarps / wpt) + warp / wpt;
+  const int part = warp % wpt;
+  if (t >= a.tokens) return;
+  const int j = lane % L, sub = lane / L;
+  pdl_wait();
+  Vec8<T> in[U];
+  // row groups part, part + wpt, ... of a token's heads
+  auto ask = [&](const T* p, long long hs, int heads, int g0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = (g0 + u * wpt) * HPI + sub;
+      if (r < heads) in[u].load(p + r * hs);
+    }
+  };
+  const T* qp = static_cast<const T*>(a.q) + t * a.q_ts + j * 8;
+  const T* kp = static_cast<const T*>(a.k) + t * a.k_ts + j * 8;
+  ask(qp, a.q_hs, a.heads, part);
+
   const int pairs = a.pair_end[a.axes - 1];
-  for (int i = threadIdx.x; i < tpc * pairs; i += kRopeWarps * 32) {
-    const int lt = i / pairs, p = i - lt * pairs;
-    const long long t = tok0 + lt;
-    if (t >= a.tokens) break;
+  for (int p = lane; p < pairs; p += 32) {
     int ax = 0;
     while (p >= a.pair_end[ax]) ++ax;
     const long long at = t * a.axes + ax;
@@ -117,126 +147,110 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_kernel(const __g
     const float frac = static_cast<float>(turns - rint(turns));
     float sn, cs;
     sincospif(2.0f * frac, &sn, &cs);
-    s_cs[lt][p] = make_float2(cs, sn);
+    s_cs[warp][p] = make_float2(cs, sn);
   }
-  __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int lt = warp / wpt, part = warp - lt * wpt;
-  const long long t = tok0 + lt;
-  if (t >= a.tokens) return;
-  const int j = lane % L, sub = lane / L;
-  // this lane's pairs: cos / sin, identity beyond the rotated dims
-  float cs[NA], sn[NA];
-  int partner = lane;
-  if (INTERLEAVED) {
-#pragma unroll
-    for (int i = 0; i < NA; ++i) {
-      const int p = 4 * j + i;
-      const float2 c = p < pairs ? s_cs[lt][p] : make_float2(1.0f, 0.0f);
-      cs[i] = c.x;
-      sn[i] = c.y;
-    }
-  } else {
-    // pairs % 8 == 0: a lane's 8 dims are all first halves, all second halves or none
-    const int hl = pairs / 8;  // lanes of one half
-    const bool first = j < hl, second = !first && j < 2 * hl;
-    partner = first ? lane + hl : second ? lane - hl : lane;
-#pragma unroll
-    for (int i = 0; i < NA; ++i) {
-      float2 c = make_float2(1.0f, 0.0f);
-      if (first || second) c = s_cs[lt][(first ? j : j - hl) * 8 + i];
-      cs[i] = c.x;
-      sn[i] = first ? -c.y : c.y;  // first: a cos - b sin, second: b cos + a sin
-    }
-  }
-  float wq[8], wk[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    wq[i] = NORM && a.qw ? a.qw[j * 8 + i] : 1.0f;
-    wk[i] = NORM && a.kw ? a.kw[j * 8 + i] : 1.0f;
-  }
-  long long slot_off = 0;  // element offset of head 0 of the token's slot in the pages
-  long long slot_hs = 0;
+  long long slot_off = 0, slot_hs = 0;  // element offset of head 0 of the token's slot in the pages
   bool stored = true;
   if (a.slots) {
-    const long long s = a.slots[t];
+    const int s = a.slots[t];
     stored = s >= 0 && s < a.n_slots;
-    const long long page = s / a.page_tokens;
-    slot_off = (page * a.kv_heads * a.page_tokens + (s - page * a.page_tokens)) * D;
+    const int page = s / a.page_tokens;
+    slot_off = (static_cast<long long>(page) * a.kv_heads * a.page_tokens + (s - page * a.page_tokens)) * D;
     slot_hs = static_cast<long long>(a.page_tokens) * D;
   }
-  const int rows = a.heads + a.kv_heads;
-  const T* qp = static_cast<const T*>(a.q) + t * a.q_ts + j * 8;
-  const T* kp = static_cast<const T*>(a.k) + t * a.k_ts + j * 8;
-  T* qo = static_cast<T*>(a.q_out) + t * a.qo_ts + j * 8;
-  T* ko = static_cast<T*>(a.k_out) + (a.slots ? slot_off : t * a.ko_ts) + j * 8;
-  const long long ko_hs = a.slots ? slot_hs : a.ko_hs;
-  constexpr int U = 4;  // row groups in flight
-  for (int r0 = part * HPI * U; r0 < rows; r0 += wpt * HPI * U) {
-    raw in[U];
+  __syncwarp();
+  // half-split: pairs % 8 == 0, a lane's 8 dims are all first halves, all second halves or none
+  const int hl = pairs / 8;  // lanes of one half
+  const int side = INTERLEAVED ? 0 : j < hl ? -1 : j < 2 * hl ? 1 : 0;
+  const int partner = lane - side * hl;
+
+  auto pass = [&](const T* src, long long hs, T* dst, long long dst_hs, int heads, const float* weight, bool keep,
+                  bool asked) {
+    uint64_t fa[4], fb[4];
+    {
+      float w[8], wo[8];  // of this lane's elements, of their partners
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * HPI + sub;
-      if (r < rows)
-        in[u] = *reinterpret_cast<const raw*>(r < a.heads ? qp + r * a.q_hs : kp + (r - a.heads) * a.k_hs);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * HPI + sub;
-      if (r0 + u * HPI >= rows) break;  // warp-uniform
-      const bool is_q = r < a.heads;
-      float x[8];
-      if (r < rows) {
-        V::unpack(in[u], x);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+      for (int i = 0; i < 8; ++i) w[i] = wo[i] = 1.0f;
+      if (NORM && weight) {
+        const float4* p = reinterpret_cast<const float4*>(weight + j * 8);
+        const float4* o = reinterpret_cast<const float4*>(weight + (j - side * hl) * 8);
+        const float4 x = p[0], y = p[1], z = o[0], v = o[1];
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w, w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
+        wo[0] = z.x, wo[1] = z.y, wo[2] = z.z, wo[3] = z.w, wo[4] = v.x, wo[5] = v.y, wo[6] = v.z, wo[7] = v.w;
       }
-      if (NORM) {
-        float ss = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float rs = rsqrtf(ss * (1.0f / D) + a.eps);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * rs * (is_q ? wq[i] : wk[i]);
-      }
-      float y[8];
-      if (INTERLEAVED) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          y[2 * i] = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i];
-          y[2 * i + 1] = x[2 * i + 1] * cs[i] + x[2 * i] * sn[i];
+      for (int i = 0; i < 4; ++i) {
+        if (INTERLEAVED) {
+          const int p = 4 * j + i;
+          const float2 c = p < pairs ? s_cs[warp][p] : make_float2(1.0f, 0.0f);
+          fa[i] = pair_f32(w[2 * i] * c.x, w[2 * i + 1] * c.x);
+          fb[i] = pair_f32(-w[2 * i + 1] * c.y, w[2 * i] * c.y);
+        } else {
+          float2 c = make_float2(1.0f, 0.0f), d = c;
+          if (side) {
+            c = s_cs[warp][(side < 0 ? j : j - hl) * 8 + 2 * i];
+            d = s_cs[warp][(side < 0 ? j : j - hl) * 8 + 2 * i + 1];
+          }
+          fa[i] = pair_f32(w[2 * i] * c.x, w[2 * i + 1] * d.x);
+          fb[i] = pair_f32(side * wo[2 * i] * c.y, side * wo[2 * i + 1] * d.y);  // a cos - b sin, b cos + a sin
         }
-        if (4 * j + 3 >= pairs) {  // pass-through dims keep their value, NaN neighbours or not
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (4 * j + i >= pairs) {
-              y[2 * i] = x[2 * i];
-              y[2 * i + 1] = x[2 * i + 1];
-            }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float other = __shfl_sync(0xffffffffu, x[i], partner);
-          y[i] = partner == lane ? x[i] : x[i] * cs[i] + other * sn[i];
-        }
-      }
-      if (r < rows) {
-        if (is_q)
-          *reinterpret_cast<raw*>(qo + r * a.qo_hs) = V::pack(y);
-        else if (stored)
-          *reinterpret_cast<raw*>(ko + (r - a.heads) * ko_hs) = V::pack(y);
       }
     }
-  }
+    for (int g0 = part; g0 * HPI < heads; g0 += U * wpt) {
+      if (g0 != part || !asked) ask(src, hs, heads, g0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r0 = (g0 + u * wpt) * HPI, r = r0 + sub;
+        if (r0 >= heads) break;  // warp-uniform
+        uint64_t scale = pair_f32(1.0f, 1.0f);
+        if (NORM) {
+          uint64_t sq = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sq = fma_f32x2(in[u].pair(i), in[u].pair(i), sq);
+          const float2 s2 = unpair_f32(sq);
+          float ss = s2.x + s2.y;
+#pragma unroll
+          for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float rs = rsqrtf(ss * (1.0f / D) + a.eps);
+          scale = pair_f32(rs, rs);
+        }
+        Vec8<T> out;
+        if (INTERLEAVED) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint64_t x = in[u].pair(i);
+            const float2 f = unpair_f32(x);
+            uint64_t y = mul_f32x2(x, fa[i]);
+            if (4 * j + i < pairs) y = fma_f32x2(pair_f32(f.y, f.x), fb[i], y);
+            out.set(i, NORM ? mul_f32x2(y, scale) : y);
+          }
+        } else {
+          const Vec8<T> other = in[u].of_lane(partner);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint64_t y = mul_f32x2(in[u].pair(i), fa[i]);
+            if (side) y = fma_f32x2(other.pair(i), fb[i], y);
+            out.set(i, NORM ? mul_f32x2(y, scale) : y);
+          }
+        }
+        if (r < heads && keep) out.store(dst + r * dst_hs);
+      }
+    }
+  };
+  pass(qp, a.q_hs, static_cast<T*>(a.q_out) + t * a.qo_ts + j * 8, a.qo_hs, a.heads, a.qw, true, true);
+  pass(kp, a.k_hs, static_cast<T*>(a.k_out) + (a.slots ? slot_off : t * a.ko_ts) + j * 8, a.slots ? slot_hs : a.ko_hs,
+       a.kv_heads, a.kw, stored, false);
   if (a.slots && stored) {
     const T* vp = static_cast<const T*>(a.v) + t * a.v_ts + j * 8;
     T* vo = static_cast<T*>(a.v_out) + slot_off + j * 8;
-    for (int r = part * HPI + sub; r < a.kv_heads; r += wpt * HPI)
-      *reinterpret_cast<raw*>(vo + r * slot_hs) = *reinterpret_cast<const raw*>(vp + r * a.v_hs);
+    for (int g0 = part; g0 * HPI < a.kv_heads; g0 += U * wpt) {
+      ask(vp, a.v_hs, a.kv_heads, g0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = (g0 + u * wpt) * HPI + sub;
+        if (r < a.kv_heads) in[u].store(vo + r * slot_hs);
+      }
+    }
   }
 }
 
@@ -302,6 +316,8 @@ extern "C" int oasis_qk_norm_rope(const oasis_qk_norm_rope_t* p, cudaStream_t st
   } else if (!p->k_out) {
     return fail(OASIS_ERR_INVALID_ARG, std::string(who) + ": null pointer");
   }
+  if ((p->q_weight && !aligned16(p->q_weight)) || (p->k_weight && !aligned16(p->k_weight)))
+    return fail(OASIS_ERR_ALIGNMENT, std::string(who) + ": weights must be 16-byte aligned");
   const int esize = p->dtype == OASIS_DT_FP32 ? 4 : 2;
   const long long strides[] = {p->q_token_stride, p->q_head_stride, p->k_token_stride, p->k_head_stride,
                                p->q_out_token_stride, p->q_out_head_stride,
@@ -327,10 +343,12 @@ extern "C" int oasis_qk_norm_rope(const oasis_qk_norm_rope_t* p, cudaStream_t st
   a.slots = append ? p->slots : nullptr;
   a.page_tokens = append ? p->pages->page_tokens : 1;
   a.n_slots = append ? static_cast<long long>(p->pages->pages) * p->pages->page_tokens : 0;
-  // few tokens: several warps share one, so that the heads of a token run side by side
+  // few tokens: several warps share one, so that its heads run side by side; a warp has a group of
+  // heads at least (4,609 tokens of 32 fp32 heads x 128: 29.5 us with two warps, 35 with one)
+  const int groups = (std::max(p->heads, p->kv_heads) * d + 255) / 256;
   a.warps_per_token = 1;
-  while (a.warps_per_token < kRopeWarps &&
-         static_cast<long long>(p->tokens) * a.warps_per_token < 16LL * num_sms())
+  while (2 * a.warps_per_token <= std::min(kRopeWarps, groups) &&
+         static_cast<long long>(p->tokens) * a.warps_per_token < 48LL * num_sms())
     a.warps_per_token *= 2;
   cudaError_t e;
   if (p->dtype == OASIS_DT_BF16)
