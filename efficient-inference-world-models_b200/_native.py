@@ -182,6 +182,16 @@ def lib() -> ctypes.CDLL:
     return _LIB
 
 
+def packed_call(name: str):
+    """The entry point ``name(const struct*, cudaStream_t)`` taking its argument struct as packed
+    bytes and the stream as an integer: a third of the host time of filling a ctypes Structure of
+    40 fields (3 against 9 microseconds)."""
+    lib()  # fail loudly if the library is missing
+    fn = getattr(ctypes.CDLL(LIB_PATH), name)  # a function object of its own, with its own argtypes
+    fn.restype, fn.argtypes = c_int, [c_char_p, c_void_p]
+    return fn
+
+
 def check(status: int) -> None:
     if status != 0:
         msg = lib().oasis_last_error().decode(errors="replace")

@@ -23,7 +23,7 @@ The reference keeps whole tensors per session and concatenates each new frame
 from __future__ import annotations
 
 import ctypes
-import math
+import struct
 import weakref
 from typing import Dict, List, Optional, Sequence, Tuple, Union
 
@@ -34,13 +34,28 @@ from . import _native as N
 from .kv_cache import HEAD_DIM, HEADS
 
 _DTYPES = {torch.bfloat16: N.DT_BF16, torch.float16: N.DT_FP16, torch.float32: N.DT_FP32}
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+_BIG = 0x3fffffff
+
+# the argument structs of include/oasis_b200.h, in native layout
+_ROPE = struct.Struct("@5P10q7if3PiP5iPP")
+_ATTN = struct.Struct("@3P4q2P5iPi2P8if")
+_entries: dict = {}
 
 
-def _current_stream(device_index: int) -> int:
-    if _raw_stream is not None:
-        return _raw_stream(device_index)
-    return torch.cuda.current_stream(device_index).cuda_stream
+def _entry(name: str):
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = N.packed_call(name)
+    return fn
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+# Every function first looks at its arguments with one cheap condition; where that does not
+# hold, the checks below find out why (or that all is well after all).
 
 
 def _elsewhere(device: torch.device, stream) -> Optional[object]:
@@ -104,24 +119,23 @@ def rope_axis_freqs(axes: Sequence[int], theta: Union[float, Sequence[float]] = 
     return torch.from_numpy(np.concatenate(parts)).to(device)
 
 
-def _rope_call(q, k, v, positions, freqs, q_out, k_out, pages, slots, q_weight, k_weight, axes,
-               interleaved, norm, eps) -> None:
+def _rope_checks(q, k, v, positions, freqs, q_weight, k_weight, axes, norm, k_pages, v_pages, slots) -> None:
+    _heads3("q", q)
+    _heads3("k", k)
+    _cuda("q", q)
     dev = q.device
-    tokens, heads, d = q.shape
-    kv_heads = k.shape[1]
+    _cuda("k", k, dev)
+    tokens, _, d = q.shape
     if k.shape[0] != tokens or k.shape[2] != d or k.dtype != q.dtype:
         raise ValueError("q and k must agree in tokens, head_dim and type")
-    dt = _DTYPES.get(q.dtype)
-    if dt is None:
+    if q.dtype not in _DTYPES:
         raise ValueError("q and k must be bf16, fp16 or fp32")
-    _cuda("k", k, dev)
     n_axes = len(axes)
     if not 1 <= n_axes <= N.MAX_AXES:
         raise ValueError("1 to 4 position axes")
-    if positions.dim() == 1 and n_axes == 1:
-        positions = positions.unsqueeze(1)
-    if (positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (tokens, n_axes)
-            or not positions.is_contiguous()):
+    shape = tuple(positions.shape)
+    if (positions.dtype not in (torch.int32, torch.int64) or not positions.is_contiguous()
+            or not (shape == (tokens, n_axes) or (n_axes == 1 and shape == (tokens,)))):
         raise ValueError(f"positions must be contiguous int32 or int64 [{tokens}][{n_axes}]")
     _cuda("positions", positions, dev)
     if freqs.dtype != torch.float64 or freqs.dim() != 1 or 2 * freqs.shape[0] != sum(axes) or not freqs.is_contiguous():
@@ -134,30 +148,85 @@ def _rope_call(q, k, v, positions, freqs, q_out, k_out, pages, slots, q_weight, 
             if w.dtype != torch.float32 or tuple(w.shape) != (d,) or not w.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous fp32 tensor [{d}]")
             _cuda(name, w, dev)
+    if v is not None:
+        _heads3("v", v)
+        if v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError("v must have k's shape and type")
+        _cuda("v", v, dev)
+        _pages(k_pages, v_pages, (4,))
+        _cuda("k_pages", k_pages, dev)
+        _cuda("v_pages", v_pages, dev)
+        if k_pages.shape[1] != k.shape[1] or k_pages.shape[3] != d or k_pages.dtype != k.dtype:
+            raise ValueError("the pages do not fit the keys (kv_heads, head_dim, type)")
+        _index32("slots", slots, (tokens,), dev)
     _no_grad(q, k, v, q_weight, k_weight)
-    qs, ks, qos = q.stride(), k.stride(), q_out.stride()
-    vs = v.stride() if v is not None else (0, 0)
-    kos = k_out.stride() if k_out is not None else (0, 0)
-    args = N.QkNormRope(
-        q.data_ptr(), k.data_ptr(), v.data_ptr() if v is not None else None, q_out.data_ptr(),
-        k_out.data_ptr() if k_out is not None else None, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], qos[0], qos[1],
-        kos[0], kos[1], tokens, heads, kv_heads, d, dt, norm, interleaved, eps,
-        q_weight.data_ptr() if q_weight is not None else None,
-        k_weight.data_ptr() if k_weight is not None else None, positions.data_ptr(),
-        positions.dtype == torch.int64, freqs.data_ptr(), n_axes, tuple(axes),
-        ctypes.pointer(pages) if pages is not None else None, slots.data_ptr() if slots is not None else None)
-    N.check(N.lib().oasis_qk_norm_rope(args, _current_stream(dev.index)))
 
 
-def _rope_out(name: str, out: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
-    if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+def _out_check(name: str, out: torch.Tensor, like: torch.Tensor) -> None:
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{name} must have its input's shape, type and device")
     _heads3(name, out)
     if out.data_ptr() == like.data_ptr() and out.stride() != like.stride():
         raise ValueError(f"{name} over its input must have the input's strides")
-    return out
+
+
+def _rope(q, k, v, positions, freqs, k_pages, v_pages, slots, axes, interleaved, norm, q_weight, k_weight, eps,
+          q_out, k_out):
+    dev, dt = q.get_device(), q.dtype
+    qh, kh, ph = q.shape, k.shape, positions.shape
+    n_axes, pt = len(axes), positions.dtype
+    fine = (dev >= 0 and dev == k.get_device() == positions.get_device() == freqs.get_device()
+            and len(qh) == len(kh) == 3 and qh[0] == kh[0] and qh[2] == kh[2] and dt == k.dtype and dt in _DTYPES
+            and 1 <= n_axes <= 4 and (pt is torch.int32 or pt is torch.int64) and ph == (qh[0], n_axes)
+            and freqs.dtype is torch.float64 and freqs.dim() == 1 and 2 * freqs.numel() == sum(axes)
+            and positions.is_contiguous() and freqs.is_contiguous()
+            and not (q.requires_grad or k.requires_grad) and q_weight is not None and k_weight is not None and norm
+            and q_weight.dtype is k_weight.dtype is torch.float32 and q_weight.shape == k_weight.shape == qh[2:]
+            and q_weight.get_device() == k_weight.get_device() == dev
+            and q_weight.is_contiguous() and k_weight.is_contiguous()
+            and not (q_weight.requires_grad or k_weight.requires_grad))
+    if fine and v is not None:
+        gh = k_pages.shape
+        fine = (v.get_device() == k_pages.get_device() == v_pages.get_device() == slots.get_device() == dev
+                and v.shape == kh and v.dtype == dt == k_pages.dtype == v_pages.dtype and dt is not torch.float32
+                and len(gh) == 4 and gh == v_pages.shape and gh[1] == kh[1] and gh[3] == kh[2]
+                and k_pages.is_contiguous() and v_pages.is_contiguous() and slots.dtype is torch.int32
+                and slots.shape == qh[:1] and slots.is_contiguous() and not v.requires_grad)
+    if not fine:
+        _rope_checks(q, k, v, positions, freqs, q_weight, k_weight, axes, norm, k_pages, v_pages, slots)
+    tokens, heads, d = qh
+    qs0, qs1, qs2 = q.stride()
+    ks0, ks1, ks2 = k.stride()
+    if q_out is None:
+        q_out = torch.empty(qh, dtype=dt, device=q.device)
+        os0, os1 = heads * d, d
+    else:
+        _out_check("q_out", q_out, q)
+        os0, os1, _ = q_out.stride()
+    vs0 = vs1 = vs2 = ko0 = ko1 = v_ptr = ko_ptr = pages_ptr = slots_ptr = 0
+    if v is not None:
+        vs0, vs1, vs2 = v.stride()
+        pages = N.Pages(k_pages.data_ptr(), v_pages.data_ptr(), 1, *k_pages.shape, _DTYPES[dt])
+        v_ptr, pages_ptr, slots_ptr = v.data_ptr(), ctypes.addressof(pages), slots.data_ptr()
+    else:
+        if k_out is None:
+            k_out = torch.empty(kh, dtype=dt, device=q.device)
+            ko0, ko1 = kh[1] * d, d
+        else:
+            _out_check("k_out", k_out, k)
+            ko0, ko1, _ = k_out.stride()
+        ko_ptr = k_out.data_ptr()
+    if d > 1 and (qs2 != 1 or ks2 != 1 or (v is not None and vs2 != 1)):
+        raise ValueError("q, k and v must be [tokens][heads][head_dim] with contiguous head_dim")
+    a = tuple(axes) + (0,) * (4 - n_axes)
+    status = _entry("oasis_qk_norm_rope")(_ROPE.pack(
+        q.data_ptr(), k.data_ptr(), v_ptr, q_out.data_ptr(), ko_ptr, qs0, qs1, ks0, ks1, vs0, vs1, os0, os1, ko0, ko1,
+        tokens, heads, kh[1], d, _DTYPES[dt], bool(norm), bool(interleaved), eps,
+        0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
+        positions.data_ptr(), pt is torch.int64, freqs.data_ptr(), n_axes, *a, pages_ptr, slots_ptr), _raw_stream(dev))
+    if status:
+        N.check(status)
+    return q_out, k_out
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *,
@@ -172,18 +241,14 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freq
     int64, ``freqs`` the fp64 frequencies of the pairs (:func:`rope_axis_freqs`).  Pairs are
     neighbours (``interleaved``, as the model here rotates) or halves of the rotated dims.  q_out / k_out may
     be q / k.  Returns (q_out, k_out)."""
-    _heads3("q", q)
-    _heads3("k", k)
-    _cuda("q", q)
-    there = _elsewhere(q.device, stream)
-    if there is not None:
-        with there:
-            return qk_norm_rope(q, k, positions, freqs, axes=axes, interleaved=interleaved, norm=norm,
-                                q_weight=q_weight, k_weight=k_weight, eps=eps, q_out=q_out, k_out=k_out)
-    q_out, k_out = _rope_out("q_out", q_out, q), _rope_out("k_out", k_out, k)
-    _rope_call(q, k, None, positions, freqs, q_out, k_out, None, None, q_weight, k_weight, axes, interleaved,
-               norm, eps)
-    return q_out, k_out
+    if stream is not None or q.get_device() != _current_device():
+        there = _elsewhere(q.device, stream)
+        if there is not None:
+            with there:
+                return qk_norm_rope(q, k, positions, freqs, axes=axes, interleaved=interleaved, norm=norm,
+                                    q_weight=q_weight, k_weight=k_weight, eps=eps, q_out=q_out, k_out=k_out)
+    return _rope(q, k, None, positions, freqs, None, None, None, axes, interleaved, norm, q_weight, k_weight, eps,
+                 q_out, k_out)
 
 
 def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
@@ -196,32 +261,41 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, posit
     cache pages [pages][kv_heads][page_tokens][head_dim]: token i into slot ``slots[i] = page *
     page_tokens + offset`` (int32; a token whose slot lies outside the pages, such as -1, is not stored;
     slots are distinct).  Returns q_out."""
+    if stream is not None or q.get_device() != _current_device():
+        there = _elsewhere(q.device, stream)
+        if there is not None:
+            with there:
+                return qk_norm_rope_append(q, k, v, positions, freqs, k_pages, v_pages, slots, axes=axes,
+                                           interleaved=interleaved, norm=norm, q_weight=q_weight,
+                                           k_weight=k_weight, eps=eps, q_out=q_out)
+    return _rope(q, k, v, positions, freqs, k_pages, v_pages, slots, axes, interleaved, norm, q_weight, k_weight,
+                 eps, q_out, None)[0]
+
+
+def _attn_checks(q, k_pages, v_pages, page_table, kv_len, cu_q, window, sinks, frame_tokens) -> None:
     _heads3("q", q)
-    _heads3("k", k)
-    _heads3("v", v)
     _cuda("q", q)
-    there = _elsewhere(q.device, stream)
-    if there is not None:
-        with there:
-            return qk_norm_rope_append(q, k, v, positions, freqs, k_pages, v_pages, slots, axes=axes,
-                                       interleaved=interleaved, norm=norm, q_weight=q_weight,
-                                       k_weight=k_weight, eps=eps, q_out=q_out)
-    if v.shape != k.shape or v.dtype != k.dtype:
-        raise ValueError("v must have k's shape and type")
-    _cuda("v", v, q.device)
+    dev = q.device
+    tokens, heads, d = q.shape
     _pages(k_pages, v_pages, (4,))
-    _cuda("k_pages", k_pages, q.device)
-    _cuda("v_pages", v_pages, q.device)
-    n_pages, kv_heads, page_tokens, d = k_pages.shape
-    if kv_heads != k.shape[1] or d != k.shape[2] or k_pages.dtype != k.dtype:
-        raise ValueError("the pages do not fit the keys (kv_heads, head_dim, type)")
-    _index32("slots", slots, (q.shape[0],), q.device)
-    q_out = _rope_out("q_out", q_out, q)
-    pages = N.Pages(k_pages.data_ptr(), v_pages.data_ptr(), 1, n_pages, kv_heads, page_tokens, d,
-                    _DTYPES[k_pages.dtype])
-    _rope_call(q, k, v, positions, freqs, q_out, None, pages, slots, q_weight, k_weight, axes, interleaved, norm,
-               eps)
-    return q_out
+    _cuda("k_pages", k_pages, dev)
+    _cuda("v_pages", v_pages, dev)
+    if k_pages.shape[3] != d or k_pages.dtype != q.dtype:
+        raise ValueError("the pages do not fit the queries (head_dim, type)")
+    if page_table.dim() != 2:
+        raise ValueError("page_table must be [sequences][pages]")
+    batch, width = page_table.shape
+    _index32("page_table", page_table, (batch, width), dev)
+    _index32("kv_len", kv_len, (batch,), dev)
+    if cu_q is not None:
+        _index32("cu_q", cu_q, (batch + 1,), dev)
+    elif tokens != batch:
+        raise ValueError("without cu_q there is one query per sequence")
+    if window is not None and window < 1:
+        raise ValueError("window must be at least one frame (None: no window)")
+    if sinks < 0 or frame_tokens < 1:
+        raise ValueError("sinks must be >= 0 and frame_tokens >= 1")
+    _no_grad(q, k_pages, v_pages)
 
 
 def attn_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -242,60 +316,56 @@ def attn_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, p
     ``max_q`` / ``max_kv`` (bounds on the queries and tokens of a sequence) only choose the launch.
     Rows that belong to no sequence are not written.  ``out`` may be q.  Returns out, or (out, lse)
     with lse fp32 [tokens][heads], the natural logarithm of the softmax sum."""
-    _heads3("q", q)
-    _cuda("q", q)
-    dev = q.device
-    there = _elsewhere(dev, stream)
-    if there is not None:
-        with there:
-            return attn_window(q, k_pages, v_pages, page_table, kv_len, cu_q, window=window, sinks=sinks,
-                               frame_tokens=frame_tokens, scale=scale, max_q=max_q, max_kv=max_kv, out=out,
-                               return_lse=return_lse)
-    tokens, heads, d = q.shape
-    _pages(k_pages, v_pages, (4,))
-    _cuda("k_pages", k_pages, dev)
-    _cuda("v_pages", v_pages, dev)
-    n_pages, kv_heads, page_tokens, d2 = k_pages.shape
-    if d2 != d or k_pages.dtype != q.dtype:
-        raise ValueError("the pages do not fit the queries (head_dim, type)")
-    if page_table.dim() != 2:
-        raise ValueError("page_table must be [sequences][pages]")
-    batch, width = page_table.shape
-    _index32("page_table", page_table, (batch, width), dev)
-    _index32("kv_len", kv_len, (batch,), dev)
-    if cu_q is not None:
-        _index32("cu_q", cu_q, (batch + 1,), dev)
-    elif tokens != batch:
-        raise ValueError("without cu_q there is one query per sequence")
-    if window is not None and window < 1:
-        raise ValueError("window must be at least one frame (None: no window)")
-    if sinks < 0 or frame_tokens < 1:
-        raise ValueError("sinks must be >= 0 and frame_tokens >= 1")
-    _no_grad(q, k_pages, v_pages)
+    dev = q.get_device()
+    if stream is not None or dev != _current_device():
+        there = _elsewhere(q.device, stream)
+        if there is not None:
+            with there:
+                return attn_window(q, k_pages, v_pages, page_table, kv_len, cu_q, window=window, sinks=sinks,
+                                   frame_tokens=frame_tokens, scale=scale, max_q=max_q, max_kv=max_kv, out=out,
+                                   return_lse=return_lse)
+    qh, gh, th, dt = q.shape, k_pages.shape, page_table.shape, q.dtype
+    if not (dev >= 0 and dev == k_pages.get_device() == v_pages.get_device() == page_table.get_device()
+            == kv_len.get_device() and len(qh) == 3 and len(gh) == 4 and gh == v_pages.shape and gh[3] == qh[2]
+            and dt == k_pages.dtype == v_pages.dtype and (dt is torch.bfloat16 or dt is torch.float16)
+            and len(th) == 2 and page_table.dtype is kv_len.dtype is torch.int32 and kv_len.shape == th[:1]
+            and k_pages.is_contiguous() and v_pages.is_contiguous() and page_table.is_contiguous()
+            and kv_len.is_contiguous() and q.stride(2) == 1
+            and (qh[0] == th[0] if cu_q is None else cu_q.get_device() == dev and cu_q.dtype is torch.int32
+                 and cu_q.shape == (th[0] + 1,) and cu_q.is_contiguous())
+            and (window is None or window >= 1) and sinks >= 0 and frame_tokens >= 1
+            and not (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad)):
+        _attn_checks(q, k_pages, v_pages, page_table, kv_len, cu_q, window, sinks, frame_tokens)
+    tokens, heads, d = qh
+    qs0, qs1, _ = q.stride()
     if out is None:
-        out = torch.empty((tokens, heads, d), dtype=q.dtype, device=dev)
+        out = torch.empty(qh, dtype=dt, device=q.device)
+        os0, os1 = heads * d, d
     else:
-        out = _rope_out("out", out, q)
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=dev) if return_lse else None
-    big = 0x3fffffff
-    qs, os_ = q.stride(), out.stride()
-    args = N.AttnWindow(
-        q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None, qs[0], qs[1], os_[0], os_[1],
-        k_pages.data_ptr(), v_pages.data_ptr(), n_pages, kv_heads, page_tokens, d, _DTYPES[q.dtype],
-        page_table.data_ptr(), width, kv_len.data_ptr(), cu_q.data_ptr() if cu_q is not None else None, batch, tokens,
-        heads, min(max_q or 0, big), min(max_kv or 0, big), min(window or 0, big), min(sinks, big),
-        min(frame_tokens, big), d ** -0.5 if scale is None else scale)
-    N.check(N.lib().oasis_attn_window(args, _current_stream(dev.index)))
+        _out_check("out", out, q)
+        os0, os1, _ = out.stride()
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    status = _entry("oasis_attn_window")(_ATTN.pack(
+        q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), qs0, qs1, os0, os1, k_pages.data_ptr(),
+        v_pages.data_ptr(), *gh, _DTYPES[dt], page_table.data_ptr(), th[1], kv_len.data_ptr(),
+        0 if cu_q is None else cu_q.data_ptr(), th[0], tokens, heads, min(max_q or 0, _BIG), min(max_kv or 0, _BIG),
+        min(window or 0, _BIG), min(sinks, _BIG), min(frame_tokens, _BIG), d ** -0.5 if scale is None else scale),
+        _raw_stream(dev))
+    if status:
+        N.check(status)
     return (out, lse) if return_lse else out
 
 
 _int32_p = ctypes.POINTER(ctypes.c_int32)
 
 
-def _page_list(name: str, x) -> np.ndarray:
+def _page_list(name: str, x):
+    """(an object that keeps the list, its address, its length) of int32 page numbers."""
     if isinstance(x, torch.Tensor):
         if x.is_cuda:
             raise ValueError(f"{name} must be on the host: it is checked before the launch")
+        if x.dtype is torch.int32 and x.dim() == 1 and x.is_contiguous():
+            return x, x.data_ptr(), x.numel()
         x = x.numpy()
     x = np.asarray(x)
     if x.size == 0:
@@ -303,10 +373,11 @@ def _page_list(name: str, x) -> np.ndarray:
     if x.ndim != 1 or x.dtype.kind not in "iu":
         raise ValueError(f"{name} must be a list of page numbers")
     if x.dtype != np.int32:
-        if x.max(initial=0) > 0x7fffffff or x.min(initial=0) < -1:
+        if x.size and (int(x.max()) > 0x7fffffff or int(x.min()) < 0):
             raise ValueError(f"{name}: page number out of range")
         x = x.astype(np.int32)
-    return np.ascontiguousarray(x)
+    x = np.ascontiguousarray(x)
+    return x, x.ctypes.data, x.shape[0]
 
 
 def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src, dst, *, to=None, stream=None) -> None:
@@ -315,31 +386,36 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src, dst, *, to=Non
     ``src`` and ``dst`` are host lists (or int tensors, arrays) of page numbers, free to change once the call returns.
     A page may be copied to several places; within one cache no destination may also be a source.  ``to``:
     the (k, v) pages of another cache that receives the pages."""
-    _pages(k_pages, v_pages, (4, 5))
-    _cuda("k_pages", k_pages)
-    dev = k_pages.device
-    _cuda("v_pages", v_pages, dev)
-    there = _elsewhere(dev, stream)
-    if there is not None:
-        with there:
-            return copy_pages(k_pages, v_pages, src, dst, to=to)
-    k2, v2 = (k_pages, v_pages) if to is None else to
+    dev, kh, dt = k_pages.get_device(), k_pages.shape, k_pages.dtype
+    if stream is not None or dev != _current_device():
+        there = _elsewhere(k_pages.device, stream)
+        if there is not None:
+            with there:
+                return copy_pages(k_pages, v_pages, src, dst, to=to)
+    if not (dev >= 0 and dev == v_pages.get_device() and kh == v_pages.shape and dt == v_pages.dtype
+            and 4 <= len(kh) <= 5 and (dt is torch.bfloat16 or dt is torch.float16)
+            and k_pages.is_contiguous() and v_pages.is_contiguous()):
+        _cuda("k_pages", k_pages)
+        _cuda("v_pages", v_pages, k_pages.device)
+        _pages(k_pages, v_pages, (4, 5))
     if to is not None:
+        k2, v2 = to
         _pages(k2, v2, (4, 5))
-        _cuda("to", k2, dev)
-        _cuda("to", v2, dev)
-        if (k2.dim() != k_pages.dim() or k2.dtype != k_pages.dtype or k2.shape[-3:] != k_pages.shape[-3:]
-                or k2.shape[:-4] != k_pages.shape[:-4]):
+        _cuda("to", k2, k_pages.device)
+        _cuda("to", v2, k_pages.device)
+        if k2.dim() != len(kh) or k2.dtype != dt or k2.shape[-3:] != kh[-3:] or k2.shape[:-4] != kh[:-4]:
             raise ValueError("the caches' pages differ")
-    src, dst = _page_list("src", src), _page_list("dst", dst)
-    if src.shape != dst.shape:
+    src, src_ptr, n = _page_list("src", src)
+    dst, dst_ptr, m = _page_list("dst", dst)
+    if n != m:
         raise ValueError("src and dst must have the same length")
-    layers = k_pages.shape[0] if k_pages.dim() == 5 else 1
-    tail = (*k_pages.shape[-3:], _DTYPES[k_pages.dtype])
-    a = N.Pages(k_pages.data_ptr(), v_pages.data_ptr(), layers, k_pages.shape[-4], *tail)
-    b = a if to is None else N.Pages(k2.data_ptr(), v2.data_ptr(), layers, k2.shape[-4], *tail)
-    N.check(N.lib().oasis_pages_copy(a, b, src.ctypes.data_as(_int32_p), dst.ctypes.data_as(_int32_p), src.shape[0],
-                                     _current_stream(dev.index)))
+    layers = kh[0] if len(kh) == 5 else 1
+    a = N.Pages(k_pages.data_ptr(), v_pages.data_ptr(), layers, *kh[-4:], _DTYPES[dt])
+    b = a if to is None else N.Pages(k2.data_ptr(), v2.data_ptr(), layers, *k2.shape[-4:], _DTYPES[dt])
+    status = N.lib().oasis_pages_copy(a, b, ctypes.cast(src_ptr, _int32_p), ctypes.cast(dst_ptr, _int32_p), n,
+                                      _raw_stream(dev))
+    if status:
+        N.check(status)
 
 
 class PagedBatchB200:

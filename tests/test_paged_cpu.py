@@ -282,3 +282,16 @@ def test_paged_struct_layouts_match_header(pkg):
             n.QkNormRope.pages.offset, ctypes.sizeof(n.QkNormRope)) == (120, 152, 196, 216, 232)
     assert (n.AttnWindow.k.offset, n.AttnWindow.page_table.offset, n.AttnWindow.cu_q.offset,
             n.AttnWindow.scale.offset, ctypes.sizeof(n.AttnWindow)) == (56, 96, 120, 160, 168)
+    # the packed forms that the functions send are the same layouts
+    fields = list(range(1, len(n.AttnWindow._fields_)))
+    raw = pkg.paged._ATTN.pack(*fields, 0.5)
+    back = n.AttnWindow.from_buffer_copy(raw + bytes(4))
+    assert [getattr(back, f[0]) for f in n.AttnWindow._fields_] == fields + [0.5]
+    names = [f[0] for f in n.QkNormRope._fields_]
+    want = {f: i + 1 for i, f in enumerate(names)}
+    want.update(eps=0.25, axis_dims=[7, 8, 9, 10], pages=0)
+    flat = [x for f in names for x in (want[f] if f == "axis_dims" else [want[f]])]
+    back = n.QkNormRope.from_buffer_copy(pkg.paged._ROPE.pack(*flat))
+    got = {f: getattr(back, f) for f in names}
+    got.update(axis_dims=list(back.axis_dims), pages=0 if not back.pages else 1)
+    assert got == want
