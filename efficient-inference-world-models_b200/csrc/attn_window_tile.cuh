@@ -515,18 +515,22 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       // Q rows of this warp into the swizzled tile, zeros past the end
       uint8_t* q_tile = sQ + i * S::kTile;
       constexpr int kChunks = D / 8;
+      uint4 qv[kChunks];  // all loads before the first store, which the compiler could not tell apart
+#pragma unroll
+      for (int x = 0; x < kChunks; ++x) {
+        const int c = x * 32 + lane;
+        const int qrow = row0 + i * kWtRows + quarter * 32 + c / kChunks;
+        qv[x] = make_uint4(0, 0, 0, 0);
+        if (qrow < row1)
+          qv[x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
+                                                  static_cast<long long>(seq.q0 + a.by_group.div(qrow)) * a.q_ts +
+                                                  (kvh * a.group + a.by_group.mod(qrow)) * a.q_hs + c % kChunks * 8);
+      }
 #pragma unroll
       for (int x = 0; x < kChunks; ++x) {
         const int c = x * 32 + lane;
         const int rr = quarter * 32 + c / kChunks, ch = c % kChunks;
-        const int qrow = row0 + i * kWtRows + rr;
-        uint4 val = make_uint4(0, 0, 0, 0);
-        if (qrow < row1) {
-          const T* src = static_cast<const T*>(a.q) + static_cast<long long>(seq.q0 + a.by_group.div(qrow)) * a.q_ts +
-                         (kvh * a.group + a.by_group.mod(qrow)) * a.q_hs + ch * 8;
-          val = *reinterpret_cast<const uint4*>(src);
-        }
-        *reinterpret_cast<uint4*>(q_tile + (ch >> 3) * S::kHalf + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = val;
+        *reinterpret_cast<uint4*>(q_tile + (ch >> 3) * S::kHalf + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = qv[x];
       }
       fence_async_smem_cta();
       __syncwarp();
@@ -748,11 +752,17 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         const float sl2 = a.scale_log2;
         for (int e = threadIdx.x * splits + rank; e < (row1 - row0) * (D / 8); e += splits * 256) {
           const int r = e / (D / 8), ch = e % (D / 8) * 2;
-          float mx[kWinSplits], top = -INFINITY;  // all loads in flight at once
+          float mx[kWinSplits], ls[kWinSplits], top = -INFINITY;
+          float4 p[kWinSplits], q[kWinSplits];
 #pragma unroll
-          for (int x = 0; x < kWinSplits; ++x) {
+          for (int x = 0; x < kWinSplits; ++x) {  // all loads in flight at once
             mx[x] = -INFINITY;
-            if (x < splits) mx[x] = ld_cluster(mapa_shared(smem_u32(part_m + r), x));
+            if (x < splits) {
+              mx[x] = ld_cluster(mapa_shared(smem_u32(part_m + r), x));
+              ls[x] = ld_cluster(mapa_shared(smem_u32(part_l + r), x));
+              p[x] = ld_cluster4(mapa_shared(smem_u32(part_o + r * D + ((ch ^ (r & 7)) << 2)), x));
+              q[x] = ld_cluster4(mapa_shared(smem_u32(part_o + r * D + (((ch + 1) ^ (r & 7)) << 2)), x));
+            }
           }
 #pragma unroll
           for (int x = 0; x < kWinSplits; ++x) top = max3_nan(top, mx[x], mx[x]);
@@ -762,11 +772,9 @@ __global__ void __launch_bounds__(kWtThreads, 1)
           for (int x = 0; x < kWinSplits; ++x) {
             if (x >= splits) continue;
             const float f = mx[x] == -INFINITY ? 0.0f : ex2((mx[x] - top) * sl2);
-            const float4 p = ld_cluster4(mapa_shared(smem_u32(part_o + r * D + ((ch ^ (r & 7)) << 2)), x));
-            const float4 q = ld_cluster4(mapa_shared(smem_u32(part_o + r * D + (((ch + 1) ^ (r & 7)) << 2)), x));
-            sum += f * ld_cluster(mapa_shared(smem_u32(part_l + r), x));
-            u.x = fmaf(f, p.x, u.x), u.y = fmaf(f, p.y, u.y), u.z = fmaf(f, p.z, u.z), u.w = fmaf(f, p.w, u.w);
-            v.x = fmaf(f, q.x, v.x), v.y = fmaf(f, q.y, v.y), v.z = fmaf(f, q.z, v.z), v.w = fmaf(f, q.w, v.w);
+            sum += f * ls[x];
+            u.x = fmaf(f, p[x].x, u.x), u.y = fmaf(f, p[x].y, u.y), u.z = fmaf(f, p[x].z, u.z), u.w = fmaf(f, p[x].w, u.w);
+            v.x = fmaf(f, q[x].x, v.x), v.y = fmaf(f, q[x].y, v.y), v.z = fmaf(f, q[x].z, v.z), v.w = fmaf(f, q[x].w, v.w);
           }
           const bool none = sum == 0.0f;
           const float inv = none ? 0.0f : 1.0f / sum;

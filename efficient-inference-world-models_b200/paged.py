@@ -35,6 +35,7 @@ from .kv_cache import HEAD_DIM, HEADS
 
 _DTYPES = {torch.bfloat16: N.DT_BF16, torch.float16: N.DT_FP16, torch.float32: N.DT_FP32}
 _BIG = 0x3fffffff
+_CONTIGUOUS = torch.contiguous_format
 
 # the argument structs of include/oasis_b200.h, in native layout
 _ROPE = struct.Struct("@5P10q7if3PiP5iPP")
@@ -198,7 +199,7 @@ def _rope(q, k, v, positions, freqs, k_pages, v_pages, slots, axes, interleaved,
     qs0, qs1, qs2 = q.stride()
     ks0, ks1, ks2 = k.stride()
     if q_out is None:
-        q_out = torch.empty(qh, dtype=dt, device=q.device)
+        q_out = torch.empty_like(q, memory_format=_CONTIGUOUS)
         os0, os1 = heads * d, d
     else:
         _out_check("q_out", q_out, q)
@@ -210,7 +211,7 @@ def _rope(q, k, v, positions, freqs, k_pages, v_pages, slots, axes, interleaved,
         v_ptr, pages_ptr, slots_ptr = v.data_ptr(), ctypes.addressof(pages), slots.data_ptr()
     else:
         if k_out is None:
-            k_out = torch.empty(kh, dtype=dt, device=q.device)
+            k_out = torch.empty_like(k, memory_format=_CONTIGUOUS)
             ko0, ko1 = kh[1] * d, d
         else:
             _out_check("k_out", k_out, k)
@@ -339,7 +340,7 @@ def attn_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, p
     tokens, heads, d = qh
     qs0, qs1, _ = q.stride()
     if out is None:
-        out = torch.empty(qh, dtype=dt, device=q.device)
+        out = torch.empty_like(q, memory_format=_CONTIGUOUS)
         os0, os1 = heads * d, d
     else:
         _out_check("out", out, q)
