@@ -249,11 +249,14 @@ int tile_splits(long long pairs, long long keys) {
 
 template <typename T, int D, int NR>
 int launch_attn_window_few(const WinArgs& a, int max_kv, cudaStream_t stream) {
-  // CTAs per (sequence, key head): enough for four full waves, while a warp keeps 8 steps of 16 keys
+  // CTAs per (sequence, key head): six per SM, where three (D = 128) are resident at a time, so that
+  // ragged sequences even out; a warp keeps a step of 16 keys at least.  32 ragged sequences of 8 key
+  // heads: 151 us with 4, 164 with 2 or 8, 187 with 1.
   const long long base = static_cast<long long>(a.batch) * a.kv_heads;
   const long long steps = (visible_keys(a, max_kv) + 15) / 16;
-  int splits = 1;
-  while (splits < kWinSplits && base * splits < 12LL * num_sms() && steps > splits * kFewWarps) splits *= 2;
+  const long long want = (6LL * num_sms() + base - 1) / base;
+  const int splits = static_cast<int>(std::max(1LL, std::min({want, (steps + kFewWarps - 1) / kFewWarps,
+                                                              static_cast<long long>(kWinSplits)})));
   cudaError_t e = launch_pdl_cluster(attn_window_few_kernel<T, D, NR>, dim3(splits * a.kv_heads, 1, a.batch),
                                      dim3(kFewWarps * 32), 0, stream, splits, a, splits);
   if (e != cudaSuccess) return cuda_status(e, "attn_window_few_kernel");
