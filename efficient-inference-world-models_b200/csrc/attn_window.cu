@@ -321,6 +321,8 @@ extern "C" int oasis_attn_window(const oasis_attn_window_t* p, cudaStream_t stre
   const oasis_pages_t pages = {const_cast<void*>(p->k), const_cast<void*>(p->v), 1, p->pages, p->kv_heads,
                                p->page_tokens, p->head_dim, p->dtype};
   if (int st = pages_check(&pages, who)) return st;
+  if (static_cast<long long>(p->pages) * p->kv_heads * p->page_tokens > 0x7fffff00LL)
+    return fail(OASIS_ERR_UNSUPPORTED, std::string(who) + ": more than 2^31 rows of pages");
   for (long long s : {p->q_token_stride, p->q_head_stride, p->out_token_stride, p->out_head_stride})
     if (s % 8) return fail(OASIS_ERR_ALIGNMENT, std::string(who) + ": strides must be multiples of 16 bytes");
   if (!aligned16(p->q) || !aligned16(p->out))

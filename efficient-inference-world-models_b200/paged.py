@@ -160,13 +160,15 @@ def _rope_checks(q, k, v, positions, freqs, q_weight, k_weight, axes, norm, k_pa
         if k_pages.shape[1] != k.shape[1] or k_pages.shape[3] != d or k_pages.dtype != k.dtype:
             raise ValueError("the pages do not fit the keys (kv_heads, head_dim, type)")
         _index32("slots", slots, (tokens,), dev)
-    _no_grad(q, k, v, q_weight, k_weight)
+    _no_grad(q, k, v, q_weight, k_weight, k_pages, v_pages)
 
 
 def _out_check(name: str, out: torch.Tensor, like: torch.Tensor) -> None:
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{name} must have its input's shape, type and device")
     _heads3(name, out)
+    if any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
+        raise ValueError(f"{name} must not be an expanded tensor: its rows are one memory")
     if out.data_ptr() == like.data_ptr() and out.stride() != like.stride():
         raise ValueError(f"{name} over its input must have the input's strides")
 
@@ -192,7 +194,8 @@ def _rope(q, k, v, positions, freqs, k_pages, v_pages, slots, axes, interleaved,
                 and v.shape == kh and v.dtype == dt == k_pages.dtype == v_pages.dtype and dt is not torch.float32
                 and len(gh) == 4 and gh == v_pages.shape and gh[1] == kh[1] and gh[3] == kh[2]
                 and k_pages.is_contiguous() and v_pages.is_contiguous() and slots.dtype is torch.int32
-                and slots.shape == qh[:1] and slots.is_contiguous() and not v.requires_grad)
+                and slots.shape == qh[:1] and slots.is_contiguous()
+                and not (v.requires_grad or k_pages.requires_grad or v_pages.requires_grad))
     if not fine:
         _rope_checks(q, k, v, positions, freqs, q_weight, k_weight, axes, norm, k_pages, v_pages, slots)
     tokens, heads, d = qh
@@ -219,6 +222,12 @@ def _rope(q, k, v, positions, freqs, k_pages, v_pages, slots, axes, interleaved,
         ko_ptr = k_out.data_ptr()
     if d > 1 and (qs2 != 1 or ks2 != 1 or (v is not None and vs2 != 1)):
         raise ValueError("q, k and v must be [tokens][heads][head_dim] with contiguous head_dim")
+    if tokens == 1:  # a dimension of one element may have any stride
+        qs0 = ks0 = vs0 = os0 = ko0 = 0
+    if heads == 1:
+        qs1 = os1 = 0
+    if kh[1] == 1:
+        ks1 = vs1 = ko1 = 0
     a = tuple(axes) + (0,) * (4 - n_axes)
     status = _entry("oasis_qk_norm_rope")(_ROPE.pack(
         q.data_ptr(), k.data_ptr(), v_ptr, q_out.data_ptr(), ko_ptr, qs0, qs1, ks0, ks1, vs0, vs1, os0, os1, ko0, ko1,
@@ -345,6 +354,10 @@ def attn_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, p
     else:
         _out_check("out", out, q)
         os0, os1, _ = out.stride()
+    if tokens == 1:  # a dimension of one element may have any stride
+        qs0 = os0 = 0
+    if heads == 1:
+        qs1 = os1 = 0
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
     status = _entry("oasis_attn_window")(_ATTN.pack(
         q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), qs0, qs1, os0, os1, k_pages.data_ptr(),
@@ -395,10 +408,12 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src, dst, *, to=Non
                 return copy_pages(k_pages, v_pages, src, dst, to=to)
     if not (dev >= 0 and dev == v_pages.get_device() and kh == v_pages.shape and dt == v_pages.dtype
             and 4 <= len(kh) <= 5 and (dt is torch.bfloat16 or dt is torch.float16)
-            and k_pages.is_contiguous() and v_pages.is_contiguous()):
+            and k_pages.is_contiguous() and v_pages.is_contiguous()
+            and not (k_pages.requires_grad or v_pages.requires_grad)):
         _cuda("k_pages", k_pages)
         _cuda("v_pages", v_pages, k_pages.device)
         _pages(k_pages, v_pages, (4, 5))
+        _no_grad(k_pages, v_pages)
     if to is not None:
         k2, v2 = to
         _pages(k2, v2, (4, 5))
@@ -406,6 +421,7 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src, dst, *, to=Non
         _cuda("to", v2, k_pages.device)
         if k2.dim() != len(kh) or k2.dtype != dt or k2.shape[-3:] != kh[-3:] or k2.shape[:-4] != kh[:-4]:
             raise ValueError("the caches' pages differ")
+        _no_grad(k2, v2)
     src, src_ptr, n = _page_list("src", src)
     dst, dst_ptr, m = _page_list("dst", dst)
     if n != m:
@@ -699,6 +715,9 @@ class PagedKVCacheB200:
         its pages are copied, sharing is not kept.  Returns its number here; the other keeps its own."""
         if other is self:
             raise ValueError("adopt takes a session of another cache: fork one of this")
+        for name in ("layers", "page_tokens", "kv_heads", "head_dim", "dtype", "device"):
+            if getattr(other, name) != getattr(self, name):
+                raise ValueError(f"the caches differ in {name}")
         s = other._get(seq)
         held = [p for p in s.pages if p >= 0]
         if len(held) > len(self._free):

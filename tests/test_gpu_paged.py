@@ -470,6 +470,92 @@ def test_other_stream(pkg, cuda):
     assert torch.equal(got, want) and not torch.equal(again, want)
 
 
+def test_one_element_dimensions_and_expanded_tensors(pkg, cuda):
+    """Strides of dimensions of one element say nothing; expanded inputs are read, expanded outputs refused."""
+    q, kp, vp, table, lens, cu = attn_inputs(cuda, [1], [40], 1, 1, 64, BF, 16)
+    odd = torch.as_strided(q, (1, 1, 64), (3, 5, 1))
+    assert torch.equal(pkg.attn_window(odd, kp, vp, table, lens, cu), pkg.attn_window(q, kp, vp, table, lens, cu))
+    f = pkg.rope_axis_freqs((64,), device=cuda)
+    pos = torch.tensor([7], dtype=torch.int32, device=cuda)
+    a, b = pkg.qk_norm_rope(odd, q, pos, f, axes=(64,))
+    assert torch.equal(a, b)
+    wide = q.expand(3, 4, 64)
+    pos3 = torch.arange(3, device=cuda)[:, None]
+    a, b = pkg.qk_norm_rope(wide, q.expand(3, 1, 64), pos3, f, axes=(64,))
+    assert torch.equal(a, b.expand(3, 4, 64).contiguous())
+    with pytest.raises(ValueError, match="expanded"):
+        pkg.qk_norm_rope(wide, q.expand(3, 1, 64), pos3, f, axes=(64,), q_out=wide)
+    with pytest.raises(ValueError, match="gradient"):
+        pkg.attn_window(q, kp.requires_grad_(), vp, table, lens, cu)
+    with torch.no_grad():
+        pkg.attn_window(q, kp, vp, table, lens, cu)
+    with pytest.raises(ValueError, match="gradient"):
+        pkg.copy_pages(kp, vp, [0], [1])
+
+
+def test_calls_side_by_side(pkg, cuda):
+    """Two captured graphs and eager calls on three streams at once share nothing."""
+    cases = [attn_inputs(cuda, [1, 1], [3000, 900], 8, 2, 128, BF, 16, seed=1),
+             attn_inputs(cuda, [144], [2000], 4, 4, 64, BF, 16, seed=2),
+             attn_inputs(cuda, [300], [700], 4, 2, 128, HF, 32, seed=3)]
+    want = [pkg.attn_window(*c) for c in cases]
+    outs = [torch.empty_like(w) for w in want]
+    graphs = []
+    for c, o in zip(cases[:2], outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(5):
+                o.fill_(0)
+                o.copy_(pkg.attn_window(*c))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(device=cuda) for _ in range(3)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            outs[2].copy_(pkg.attn_window(*cases[2]))
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert torch.equal(o, w)
+    pkg._native.check(pkg.lib().oasis_check_device_error())
+
+
+FIRST_CALL = """
+import importlib, sys, torch
+sys.path[:0] = [{root!r}, {tests!r}]
+import test_gpu_paged as t
+pkg = importlib.import_module({name!r})
+dev = torch.device("cuda:0")
+pkg.lib()
+case = t.attn_inputs(dev, [144], [2000], 4, 4, 64, torch.bfloat16, 16)
+few = t.attn_inputs(dev, [1], [500], 4, 4, 64, torch.bfloat16, 16)
+k, v = (torch.nan_to_num(p) for p in case[1:3])
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = pkg.attn_window(*case)
+    one = pkg.attn_window(*few)
+    pkg.copy_pages(k, v, [0, 1], [126, 127])
+graph.replay()
+assert torch.equal(out, pkg.attn_window(*case)) and torch.equal(one, pkg.attn_window(*few))
+assert torch.equal(k[126:], k[:2]) and torch.equal(v[126:], v[:2])
+print("fine")
+"""
+
+
+def test_first_call_under_capture(pkg, cuda):
+    """A process whose first use of the operators is a capture."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = FIRST_CALL.format(root=os.path.dirname(here), tests=here, name=pkg.__name__)
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "fine" in done.stdout, done.stderr[-2000:]
+
+
 def test_session_end_to_end(pkg, cuda):
     """Sessions that grow by frames, fork, evict, compact and move, layer by layer, through the cache's
     methods and one captured graph, against attention over the whole history in 64 bits."""

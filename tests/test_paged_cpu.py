@@ -165,7 +165,10 @@ def test_cache_refusals(pkg):
             pkg.PagedKVCacheB200(**args)
     c = make(pkg)
     a = c.new()
-    for call in (lambda: c.fork(a, -1), lambda: c.truncate(a, 1), lambda: c.evict(a, 0), lambda: c.free(7),
+    others = [make(pkg, layers=3), make(pkg, dtype=torch.float16)]
+    for o in others:
+        o.new()
+    for call in (lambda: c.adopt(others[0], 0), lambda: c.adopt(others[1], 0), lambda: c.fork(a, -1), lambda: c.truncate(a, 1), lambda: c.evict(a, 0), lambda: c.free(7),
                  lambda: c.adopt(c, a)):
         with pytest.raises(ValueError):
             call()
@@ -267,7 +270,8 @@ def attn_args(pkg, **kw):
     ({"dtype": 2}, 6), ({"scale": 0.0}, 1), ({"scale": float("nan")}, 1), ({"scale": float("inf")}, 1),
     ({"batch": 65536}, 6), ({"table_width": 1 << 27}, 6), ({"cu_q": None}, 1), ({"q": None}, 1),
     ({"kv_len": None}, 1), ({"k": None}, 1), ({"v": 24}, 2), ({"out": 24}, 2), ({"q_head_stride": 68}, 2),
-    ({"pages": 0}, 1), ({"pages": 1 << 28}, 6),
+    ({"pages": 0}, 1), ({"pages": 1 << 28}, 6), ({"pages": 1 << 26, "kv_heads": 2}, 6),
+    ({"tokens": 1 << 30, "heads": 4}, 6),
 ])
 def test_attn_window_refusals(pkg, change, status):
     assert pkg.lib().oasis_attn_window(attn_args(pkg, **change), None) == status
