@@ -32,7 +32,7 @@ struct WtShape {
   static constexpr int kBars = 3 * kStages + 12;
   // D = 64 leaves TMEM columns for P beside S: the next S is then computed under the softmax
   static constexpr bool kEarly = D == 64;
-  // quarters of P that the MMAs get before the rest is there: 456 us with two against 465 with three
+  // quarters of P that the MMAs get before the rest is there: 416 us with two against 423 with three
   // for a prompt of 8,191 tokens at D = 128, 75 against 71 us for 8 sessions' frames at D = 64
   static constexpr int kHandover = kEarly ? 3 : 2;
   static constexpr int kO = 256, kP = kEarly ? kO + 2 * D : 0, kPStep = kEarly ? 64 : 128;  // columns of tile 0, 1
@@ -636,18 +636,37 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         const float base = m == -INFINITY ? 0.0f : fmaf(m, 0.0f, -m * sl2);  // NaN for a maximum of +inf
         uint64_t sum[2] = {0, 0};
         // (D = 128: the columns of P lie over those of S, which are all in registers.)  The MMAs take
-        // the first kHandover quarters of the keys while the rest is computed.
+        // the first kHandover quarters of the keys while the rest is computed.  The order in which the
+        // source has a quarter's arithmetic is the order in which it is issued: pair by pair at D = 64
+        // (8 sessions' frames 68 us, 74 in sweeps), in three sweeps at D = 128 (the prompt 416, 433 by pairs).
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
+          if (S::kEarly) {
 #pragma unroll
-          for (int x = 0; x < 32; x += 2) {
-            float2 e =
-                unpair_f32(fma_f32x2(pair_f32(v[c][x], v[c][x + 1]), pair_f32(sl2, sl2), pair_f32(base, base)));
-            e.x = ex2(e.x);
-            e.y = ex2(e.y);
-            sum[(x >> 1) & 1] = add_f32x2(sum[(x >> 1) & 1], pair_f32(e.x, e.y));
-            pk[x / 2] = pack2<T>(e.x, e.y);
+            for (int x = 0; x < 32; x += 2) {
+              float2 e =
+                  unpair_f32(fma_f32x2(pair_f32(v[c][x], v[c][x + 1]), pair_f32(sl2, sl2), pair_f32(base, base)));
+              e.x = ex2(e.x);
+              e.y = ex2(e.y);
+              sum[(x >> 1) & 1] = add_f32x2(sum[(x >> 1) & 1], pair_f32(e.x, e.y));
+              pk[x / 2] = pack2<T>(e.x, e.y);
+            }
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; x += 2) {
+              const float2 t =
+                  unpair_f32(fma_f32x2(pair_f32(v[c][x], v[c][x + 1]), pair_f32(sl2, sl2), pair_f32(base, base)));
+              v[c][x] = __float_as_uint(t.x);
+              v[c][x + 1] = __float_as_uint(t.y);
+            }
+#pragma unroll
+            for (int x = 0; x < 32; ++x) v[c][x] = __float_as_uint(ex2(__uint_as_float(v[c][x])));
+#pragma unroll
+            for (int x = 0; x < 32; x += 2) {
+              sum[(x >> 1) & 1] = add_f32x2(sum[(x >> 1) & 1], pair_f32(v[c][x], v[c][x + 1]));
+              pk[x / 2] = pack2<T>(__uint_as_float(v[c][x]), __uint_as_float(v[c][x + 1]));
+            }
           }
           if (c == S::kHandover) {
             tmem_wait_st(pk);  // of the earlier quarters, under the arithmetic of this one
