@@ -282,12 +282,19 @@ __global__ void __launch_bounds__(kWtThreads, 1)
   WtTiles tiles = wt_tiles(span, kWtKeys);
   tiles.keep(rank, splits);
   const int n = tiles.n;
-  // a split CTA's result, over the ring once it is done: O [256][D] fp32 (16-byte chunks
-  // swizzled by row), then the rows' maxima and sums
+  // The parts that the CTAs of a cluster send each other, over the ring once all are done with it:
+  // of every CTA, for this one's share of the rows, O [share][D] fp32 (16-byte chunks swizzled by
+  // row), the rows' maxima and sums, and the mark of warp 9.
+  const int share = (row1 - row0 + splits - 1) / splits;
   float* part_o = reinterpret_cast<float*>(ring);
-  float* part_m = part_o + 2 * kWtRows * D;
-  float* part_l = part_m + 2 * kWtRows;
-  static_assert(2 * kWtRows * (D + 2) * 4 <= kStages * S::kTile, "the ring holds a split's result");
+  float* part_m = part_o + splits * share * D;
+  float* part_l = part_m + splits * share;
+  uint32_t* part_mark = reinterpret_cast<uint32_t*>(part_l + splits * share);
+  static_assert((2 * kWtRows + kWinSplits) * (D + 2) * 4 + kWinSplits * 4 <= kStages * S::kTile,
+                "the ring holds a CTA's share of all parts");
+  float m = -INFINITY, l = 0.0f;  // of a softmax thread's row
+  uint32_t np = 0;
+  bool ok = true;
 
   if (warp >= 8) {
     if (row0 >= rows) {
@@ -556,9 +563,6 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         }
       }
       const bool holes = __any_sync(0xffffffffu, hole && mine.any);
-      float m = -INFINITY, l = 0.0f;
-      uint32_t np = 0;
-      bool ok = true;
       for (int j = 0; j < n; ++j) {
         const int tile = tiles.tile(j), k0 = tile * kWtKeys;
         if (!mine.some(k0, k0 + kWtKeys)) continue;
@@ -687,26 +691,10 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       if (ok && np > 0) ok = mbar_wait(&pv_done[i], (np - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      if (splits > 1) {
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // both tiles' MMAs have read the ring
-        const int rr = i * kWtRows + r;
-#pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32] = {};
-          if (np > 0) {
-            tmem_ld32_nowait(o_addr + c * 32, o);
-            tmem_wait_ld(o);
-          }
-#pragma unroll
-          for (int x = 0; x < 8; ++x)
-            *reinterpret_cast<uint4*>(part_o + rr * D + (((c * 8 + x) ^ (rr & 7)) << 2)) =
-                make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
-        }
-        part_m[rr] = ok ? m : __uint_as_float(0x7fffffffu);
-        part_l[rr] = l;
-      }
       // warp 9's mark: every tile it looked at was multiplied before pv_done
-      else if (ok && *reinterpret_cast<volatile uint32_t*>(dirty)) {
+      if (splits > 1) {
+        // joined below
+      } else if (ok && *reinterpret_cast<volatile uint32_t*>(dirty)) {
         for (int x = 0; x < 32; ++x) {
           const int rr = row0 + i * kWtRows + quarter * 32 + x;
           if (rr < row1) window_row<T, D>(a, b, seq, a.by_group.div(rr), kvh * a.group + a.by_group.mod(rr), lane);
@@ -759,48 +747,63 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         window_row<T, D>(a, b, seq, a.by_group.div(r), kvh * a.group + a.by_group.mod(r), lane);
   }
   if (splits > 1) {
-    // join the cluster's results in rank order, each CTA a share of the rows
-    cluster_sync_all();
+    // Join the cluster's parts, each CTA a share of the rows: stores into the owner's shared memory
+    // need no answer, where loads from the others waited 4 us for theirs.
+    cluster_sync_all();  // every CTA's MMAs have read its ring
     if (warp < 8 && row0 < rows) {
+      const int quarter = warp & 3, rr = (warp >> 2) * kWtRows + quarter * 32 + lane;
+      const uint32_t o_addr = tmem + S::kO + (warp >> 2) * D + (static_cast<uint32_t>(quarter * 32) << 16);
+      const int owner = min(rr / share, splits - 1), slot = rank * share + rr - owner * share;
+      const bool mine = rr < row1 - row0;
+      if (mine) {
+        st_cluster(mapa_shared(smem_u32(part_m + slot), owner), ok ? m : __uint_as_float(0x7fffffffu));
+        st_cluster(mapa_shared(smem_u32(part_l + slot), owner), l);
+      }
+      if (threadIdx.x < splits)
+        st_cluster(mapa_shared(smem_u32(part_mark + rank), threadIdx.x), __uint_as_float(*reinterpret_cast<volatile uint32_t*>(dirty)));
+      const uint32_t dst = mapa_shared(smem_u32(part_o + slot * D), owner);
+#pragma unroll 1
+      for (int c = 0; np > 0 && c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32_nowait(o_addr + c * 32, o);
+        tmem_wait_ld(o);
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          if (mine) st_cluster4(dst + (((c * 8 + x) ^ (slot & 7)) << 4), o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+      }
+    }
+    cluster_sync_all();
+    const int own0 = rank * share, own = min(share, row1 - row0 - own0);  // this CTA's rows
+    if (warp < 8 && own > 0) {
       uint32_t marked = 0;
-      for (int x = 0; x < splits; ++x) marked |= __float_as_uint(ld_cluster(mapa_shared(smem_u32(dirty), x)));
+      for (int x = 0; x < splits; ++x) marked |= part_mark[x];
       if (marked) {
-        for (int r = row0 + rank * 8 + warp; r < row1; r += splits * 8)
+        for (int r = row0 + own0 + warp; r < row0 + own0 + own; r += 8)
           window_row<T, D>(a, b, seq, a.by_group.div(r), kvh * a.group + a.by_group.mod(r), lane);
       } else {
         const float sl2 = a.scale_log2;
-        for (int e = threadIdx.x * splits + rank; e < (row1 - row0) * (D / 8); e += splits * 256) {
+        for (int e = threadIdx.x; e < own * (D / 8); e += 256) {
           const int r = e / (D / 8), ch = e % (D / 8) * 2;
-          float mx[kWinSplits], ls[kWinSplits], top = -INFINITY;
-          float4 p[kWinSplits], q[kWinSplits];
-#pragma unroll
-          for (int x = 0; x < kWinSplits; ++x) {  // all loads in flight at once
-            mx[x] = -INFINITY;
-            if (x < splits) {
-              mx[x] = ld_cluster(mapa_shared(smem_u32(part_m + r), x));
-              ls[x] = ld_cluster(mapa_shared(smem_u32(part_l + r), x));
-              p[x] = ld_cluster4(mapa_shared(smem_u32(part_o + r * D + ((ch ^ (r & 7)) << 2)), x));
-              q[x] = ld_cluster4(mapa_shared(smem_u32(part_o + r * D + (((ch + 1) ^ (r & 7)) << 2)), x));
-            }
-          }
-#pragma unroll
-          for (int x = 0; x < kWinSplits; ++x) top = max3_nan(top, mx[x], mx[x]);
+          float top = -INFINITY;
+          for (int x = 0; x < splits; ++x) top = max3_nan(top, part_m[x * share + r], part_m[x * share + r]);
           float sum = 0.0f;
           float4 u = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = u;
-#pragma unroll
-          for (int x = 0; x < kWinSplits; ++x) {
-            if (x >= splits) continue;
-            const float f = mx[x] == -INFINITY ? 0.0f : ex2((mx[x] - top) * sl2);
-            sum += f * ls[x];
-            u.x = fmaf(f, p[x].x, u.x), u.y = fmaf(f, p[x].y, u.y), u.z = fmaf(f, p[x].z, u.z), u.w = fmaf(f, p[x].w, u.w);
-            v.x = fmaf(f, q[x].x, v.x), v.y = fmaf(f, q[x].y, v.y), v.z = fmaf(f, q[x].z, v.z), v.w = fmaf(f, q[x].w, v.w);
+          for (int x = 0; x < splits; ++x) {  // in rank order
+            const int at = x * share + r;
+            if (part_m[at] == -INFINITY) continue;  // (its O was not sent)
+            const float f = ex2((part_m[at] - top) * sl2);
+            const float4 p = *reinterpret_cast<const float4*>(part_o + at * D + ((ch ^ (at & 7)) << 2));
+            const float4 q = *reinterpret_cast<const float4*>(part_o + at * D + (((ch + 1) ^ (at & 7)) << 2));
+            sum += f * part_l[at];
+            u.x = fmaf(f, p.x, u.x), u.y = fmaf(f, p.y, u.y), u.z = fmaf(f, p.z, u.z), u.w = fmaf(f, p.w, u.w);
+            v.x = fmaf(f, q.x, v.x), v.y = fmaf(f, q.y, v.y), v.z = fmaf(f, q.z, v.z), v.w = fmaf(f, q.w, v.w);
           }
           const bool none = sum == 0.0f;
           const float inv = none ? 0.0f : 1.0f / sum;
           uint4 w4 = make_uint4(pack2<T>(u.x * inv, u.y * inv), pack2<T>(u.z * inv, u.w * inv),
                                 pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
           if (none) w4 = make_uint4(0, 0, 0, 0);
-          const int qr = row0 + r, head = kvh * a.group + a.by_group.mod(qr);
+          const int qr = row0 + own0 + r, head = kvh * a.group + a.by_group.mod(qr);
           const long long tok = seq.q0 + a.by_group.div(qr);
           *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs + ch * 4) = w4;
           if (a.lse && ch == 0)
@@ -808,7 +811,6 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         }
       }
     }
-    cluster_sync_all();  // the others have read this CTA's part
   }
   tc_fence_before();
   __syncthreads();
