@@ -45,7 +45,11 @@ template <int D, int NR>
 struct alignas(16) FewShared {
   float o[kFewWarps][NR][D];
   float m[kFewWarps][NR], l[kFewWarps][NR];
-  float cm[NR], cl[NR];  // of the CTA; its O is o[0]
+  // from the CTAs of the cluster: maxima and sums of all rows, and of this CTA's share of O, 4 dims
+  // of a row at a time, unit e of the whole in place e / CTAs of CTA e % CTAs
+  float cm[kWinSplits][NR], cl[kWinSplits][NR];
+  float4 co[NR * D / 4 + kWinSplits];
+  uint32_t marks[kWinSplits];
   uint32_t dirty;
 };
 
@@ -62,6 +66,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, D == 64 ? (NR == 8 ? 4 : 3) : 
   const int split = static_cast<int>(blockIdx.x) % splits;  // rank in the cluster
   const int kvh = static_cast<int>(blockIdx.x) / splits;
   const int b = blockIdx.z;
+  if (splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA is here
   pdl_wait();
   const WinSeq seq = win_seq(a, b);
   const int rows = seq.n_q * a.group;
@@ -284,7 +289,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, D == 64 ? (NR == 8 ? 4 : 3) : 
     // weight of a partial result of maximum x under the joint maximum y
     auto weight = [&](float x, float y) { return x == -INFINITY ? 0.0f : ex2((x - y) * sl2); };
     auto join_max = [](float x, float y) { return max3_nan(x, y, y); };
-    for (int e = threadIdx.x; e < (row1 - row0) * (D / 4); e += kFewWarps * 32) {
+    // what the others may write to: the CTAs are all here, and done with an earlier turn's parts
+    if (splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    const int units = (row1 - row0) * (D / 4), share = (units + splits - 1) / splits;
+    for (int e = threadIdx.x; e < units; e += kFewWarps * 32) {
       const int r = e / (D / 4), d = (e % (D / 4)) * 4;
       float top = sh.m[0][r];
 #pragma unroll
@@ -299,43 +307,42 @@ __global__ void __launch_bounds__(kFewWarps * 32, D == 64 ? (NR == 8 ? 4 : 3) : 
         acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y);
         acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
       }
-      *reinterpret_cast<float4*>(&sh.o[0][r][d]) = acc;  // this thread alone reads these elements
-      if (d == 0) {
-        sh.cm[r] = top;
-        sh.cl[r] = sum;
-      }
+      // sent to its owner (stores need no answer, loads from the others would wait for theirs)
+      const int owner = e % splits;
+      st_cluster4(mapa_shared(smem_u32(&sh.co[split * share + e / splits]), owner), __float_as_uint(acc.x),
+                  __float_as_uint(acc.y), __float_as_uint(acc.z), __float_as_uint(acc.w));
+      if (d == 0)
+        for (int x = 0; x < splits; ++x) {
+          st_cluster(mapa_shared(smem_u32(&sh.cm[split][r]), x), top);
+          st_cluster(mapa_shared(smem_u32(&sh.cl[split][r]), x), sum);
+        }
     }
-    // ---- and CTAs of the cluster
+    if (threadIdx.x < splits)
+      st_cluster(mapa_shared(smem_u32(&sh.marks[split]), threadIdx.x),
+                 __uint_as_float(*reinterpret_cast<volatile uint32_t*>(&sh.dirty)));
+    __syncwarp();
     if (splits > 1)
       cluster_sync_all();
     else
       __syncthreads();
+    // ---- and CTAs of the cluster, in rank order
     uint32_t marked = 0;
-#pragma unroll
-    for (int x = 0; x < kWinSplits; ++x)
-      if (x < splits) marked |= __float_as_uint(ld_cluster(mapa_shared(smem_u32(&sh.dirty), x)));
+    for (int x = 0; x < splits; ++x) marked |= sh.marks[x];
     if (marked) {
       for (int r = row0 + part; r < row1; r += parts)
         window_row<T, D>(a, b, seq, a.by_group.div(r), kvh * a.group + a.by_group.mod(r), lane);
     } else {
-      for (int e = threadIdx.x * splits + split; e < (row1 - row0) * (D / 4); e += splits * kFewWarps * 32) {
+      for (int i = threadIdx.x; i * splits + split < units; i += kFewWarps * 32) {
+        const int e = i * splits + split;
         const int r = e / (D / 4), d = (e % (D / 4)) * 4;
-        float mx[kWinSplits], top = -INFINITY;  // all loads in flight at once
-#pragma unroll
-        for (int x = 0; x < kWinSplits; ++x) {
-          mx[x] = -INFINITY;
-          if (x < splits) mx[x] = ld_cluster(mapa_shared(smem_u32(&sh.cm[r]), x));
-        }
-#pragma unroll
-        for (int x = 0; x < kWinSplits; ++x) top = join_max(top, mx[x]);
+        float top = -INFINITY;
+        for (int x = 0; x < splits; ++x) top = join_max(top, sh.cm[x][r]);
         float sum = 0.0f;
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int x = 0; x < kWinSplits; ++x) {
-          if (x >= splits) continue;
-          const float f = weight(mx[x], top);
-          const float4 z = ld_cluster4(mapa_shared(smem_u32(&sh.o[0][r][d]), x));
-          sum += f * ld_cluster(mapa_shared(smem_u32(&sh.cl[r]), x));
+        for (int x = 0; x < splits; ++x) {
+          const float f = weight(sh.cm[x][r], top);
+          const float4 z = sh.co[x * share + i];
+          sum += f * sh.cl[x][r];
           acc.x = fmaf(f, z.x, acc.x), acc.y = fmaf(f, z.y, acc.y);
           acc.z = fmaf(f, z.z, acc.z), acc.w = fmaf(f, z.w, acc.w);
         }
@@ -350,11 +357,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, D == 64 ? (NR == 8 ? 4 : 3) : 
         if (a.lse && d == 0) a.lse[tok * a.heads + head] = none ? -INFINITY : (top * sl2 + log2f(sum)) * 0.6931471805599453f;
       }
     }
-    if (splits > 1)
-      cluster_sync_all();  // the others have read this CTA's part
-    else
-      __syncthreads();
+    __syncwarp();
+    if (splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // done with the parts
+    __syncthreads();
   }
+  if (splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the last arrival's
 }
 
 }  // namespace oasis

@@ -749,6 +749,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
   if (splits > 1) {
     // Join the cluster's parts, each CTA a share of the rows: stores into the owner's shared memory
     // need no answer, where loads from the others waited 4 us for theirs.
+    __syncwarp();
     cluster_sync_all();  // every CTA's MMAs have read its ring
     if (warp < 8 && row0 < rows) {
       const int quarter = warp & 3, rr = (warp >> 2) * kWtRows + quarter * 32 + lane;
@@ -772,6 +773,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
           if (mine) st_cluster4(dst + (((c * 8 + x) ^ (slot & 7)) << 4), o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
       }
     }
+    __syncwarp();
     cluster_sync_all();
     const int own0 = rank * share, own = min(share, row1 - row0 - own0);  // this CTA's rows
     if (warp < 8 && own > 0) {
