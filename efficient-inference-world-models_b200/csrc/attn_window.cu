@@ -92,12 +92,7 @@ __device__ __forceinline__ __nv_bfloat16 from_float(float x) { return __float2bf
 template <>
 __device__ __forceinline__ __half from_float(float x) { return __float2half_rn(x); }
 
-// From the shared memory of a CTA of the cluster (a mapa_shared address).
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
-  return v;
-}
+// Into the shared memory of a CTA of the cluster (a mapa_shared address).
 __device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
@@ -105,14 +100,6 @@ __device__ __forceinline__ void st_cluster4(uint32_t addr, uint32_t x, uint32_t 
   asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w)
                : "memory");
 }
-__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr));
-  return v;
-}
-
 // One query row by one warp, key after key with the running maximum and sum: each lane holds
 // D / 32 dims.  Reads only what the row sees.
 template <typename T, int D>
