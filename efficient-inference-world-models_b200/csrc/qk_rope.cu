@@ -6,23 +6,29 @@
 
 namespace oasis {
 
-// 8 consecutive elements of a row in registers: as four pairs of fp32, and back with one rounding to
-// nearest even.
+// 8 elements of a row in registers, two runs of 4: as four pairs of fp32, and back with one rounding to
+// nearest even.  TWO: the runs are apart (two accesses), otherwise they follow each other.
 template <typename T>
 struct Vec8 {
   uint32_t w[4];
-  __device__ __forceinline__ void load(const T* p) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  template <bool TWO>
+  __device__ __forceinline__ void load(const T* p, int second) {
+    if (TWO) {
+      const uint2 x = *reinterpret_cast<const uint2*>(p), y = *reinterpret_cast<const uint2*>(p + second);
+      w[0] = x.x, w[1] = x.y, w[2] = y.x, w[3] = y.y;
+    } else {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    }
   }
-  __device__ __forceinline__ void store(T* p) const {
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  __device__ __forceinline__ Vec8 of_lane(int lane) const {
-    Vec8 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.w[i] = __shfl_sync(0xffffffffu, w[i], lane);
-    return r;
+  template <bool TWO>
+  __device__ __forceinline__ void store(T* p, int second) const {
+    if (TWO) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(p + second) = make_uint2(w[2], w[3]);
+    } else {
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
   __device__ __forceinline__ uint64_t pair(int i) const;
   __device__ __forceinline__ void set(int i, uint64_t p);
@@ -50,23 +56,15 @@ __device__ __forceinline__ void Vec8<__half>::set(int i, uint64_t p) {
 template <>
 struct Vec8<float> {
   float4 a, b;
-  __device__ __forceinline__ void load(const float* p) {
-    a = reinterpret_cast<const float4*>(p)[0];
-    b = reinterpret_cast<const float4*>(p)[1];
+  template <bool TWO>
+  __device__ __forceinline__ void load(const float* p, int second) {
+    a = *reinterpret_cast<const float4*>(p);
+    b = *reinterpret_cast<const float4*>(p + (TWO ? second : 4));
   }
-  __device__ __forceinline__ void store(float* p) const {
-    reinterpret_cast<float4*>(p)[0] = a;
-    reinterpret_cast<float4*>(p)[1] = b;
-  }
-  __device__ __forceinline__ Vec8 of_lane(int lane) const {
-    Vec8 r;
-    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], lane);
-    r.a = make_float4(y[0], y[1], y[2], y[3]);
-    r.b = make_float4(y[4], y[5], y[6], y[7]);
-    return r;
+  template <bool TWO>
+  __device__ __forceinline__ void store(float* p, int second) const {
+    *reinterpret_cast<float4*>(p) = a;
+    *reinterpret_cast<float4*>(p + (TWO ? second : 4)) = b;
   }
   __device__ __forceinline__ uint64_t pair(int i) const {
     return i == 0 ? pair_f32(a.x, a.y) : i == 1 ? pair_f32(a.z, a.w) : i == 2 ? pair_f32(b.x, b.y) : pair_f32(b.z, b.w);
@@ -99,22 +97,24 @@ struct RopeArgs {
 
 constexpr int kRopeWarps = 8;
 
-// A head of D elements is spread over L = D / 8 lanes, 8 consecutive elements (16 or 32 bytes)
-// each, so a warp takes 32 / L heads at a time and a mean of squares is log2(L) shuffles.  One or,
-// where tokens are few, several warps take a token.  A warp asks for the first rows, then computes the
+// A head of D elements is spread over L = D / 8 lanes, 8 elements each, so a warp takes 32 / L heads
+// at a time and a mean of squares is log2(L) shuffles.  A lane holds whole pairs: neighbours are 8
+// consecutive elements; with the half-split pairing a lane has 4 elements of the first half of the
+// rotated dims and their 4 partners of the second (or 8 dims that are not rotated).  One or, where
+// tokens are few, several warps take a token.  A warp asks for the first rows, then computes the
 // cos and sin of the token's rotated pairs under those loads, one or more pairs per lane, and hands
 // them round through shared memory: the angle is position * frequency in turns, reduced to
 // [-1/2, 1/2] in fp64 (an fp32 angle of position 10^6 is off by 0.06 rad), then sincospi in fp32.
-// Weight and rotation of a lane's 8 elements become two factors each, kept for all heads of the
-// token:  y = rsqrt(mean) * (A x + B x'),  x' the other element of the pair (the lane's own
-// neighbour, or with the half-split pairing that of the lane rot / 16 away, which comes by shuffle as loaded).
-// Bound by HBM (every byte read and written once).
+// Weight and rotation of a lane's elements become two factors each, kept for all heads of the
+// token:  y = rsqrt(mean) * (A x + B x'),  x' the other element of the pair.
+// Bound by HBM and by instructions at once: 36,864 tokens of 32 heads x 64 (302 MB) take ROPEUS.
 template <typename T, int D, bool INTERLEAVED, bool NORM>
 __global__ void __launch_bounds__(kRopeWarps * 32, 4) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int L = D / 8;
   constexpr int HPI = 32 / L;                // heads per warp and row group
   constexpr int U = sizeof(T) == 4 ? 2 : 4;  // row groups in flight
-  __shared__ float2 s_cs[kRopeWarps][D / 2];
+  constexpr bool TWO = !INTERLEAVED;
+  __shared__ __align__(16) float s_cos[kRopeWarps][D / 2], s_sin[kRopeWarps][D / 2];
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wpt = a.warps_per_token;
@@ -122,6 +122,11 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 4) qk_norm_rope_kernel(const 
   const int part = warp % wpt;
   if (t >= a.tokens) return;
   const int j = lane % L, sub = lane / L;
+  const int pairs = a.pair_end[a.axes - 1];
+  // this lane's elements: two runs of 4 at `first` and `first + second`, rotated by pairs pair0 ..
+  const int turning = pairs / 4;  // half-split: lanes with rotated dims (pairs % 8 == 0)
+  const int first = INTERLEAVED ? 8 * j : j < turning ? 4 * j : 2 * pairs + 8 * (j - turning);
+  const int second = INTERLEAVED || j >= turning ? 4 : pairs;
   pdl_wait();
   Vec8<T> in[U];
   // row groups part, part + wpt, ... of a token's heads
@@ -129,25 +134,28 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 4) qk_norm_rope_kernel(const 
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int r = (g0 + u * wpt) * HPI + sub;
-      if (r < heads) in[u].load(p + r * hs);
+      if (r < heads) in[u].template load<TWO>(p + r * hs, second);
     }
   };
-  const T* qp = static_cast<const T*>(a.q) + t * a.q_ts + j * 8;
-  const T* kp = static_cast<const T*>(a.k) + t * a.k_ts + j * 8;
+  const T* qp = static_cast<const T*>(a.q) + t * a.q_ts + first;
+  const T* kp = static_cast<const T*>(a.k) + t * a.k_ts + first;
   ask(qp, a.q_hs, a.heads, part);
 
-  const int pairs = a.pair_end[a.axes - 1];
-  for (int p = lane; p < pairs; p += 32) {
-    int ax = 0;
-    while (p >= a.pair_end[ax]) ++ax;
-    const long long at = t * a.axes + ax;
-    const double pos = a.positions_64 ? static_cast<double>(static_cast<const int64_t*>(a.positions)[at])
-                                      : static_cast<double>(static_cast<const int32_t*>(a.positions)[at]);
-    const double turns = pos * a.freqs[p] * 0.15915494309189533577;  // 1 / (2 pi)
-    const float frac = static_cast<float>(turns - rint(turns));
-    float sn, cs;
-    sincospif(2.0f * frac, &sn, &cs);
-    s_cs[warp][p] = make_float2(cs, sn);
+  for (int p = lane; p < D / 2; p += 32) {
+    float cs = 1.0f, sn = 0.0f;
+    if (p < pairs) {
+      int ax = 0;
+#pragma unroll
+      for (int i = 0; i + 1 < OASIS_MAX_AXES; ++i) ax += i + 1 < a.axes && p >= a.pair_end[i];
+      const long long at = t * a.axes + ax;
+      const double pos = a.positions_64 ? static_cast<double>(static_cast<const int64_t*>(a.positions)[at])
+                                        : static_cast<double>(static_cast<const int32_t*>(a.positions)[at]);
+      const double turns = pos * a.freqs[p] * 0.15915494309189533577;  // 1 / (2 pi)
+      const float frac = static_cast<float>(turns - rint(turns));
+      sincospif(2.0f * frac, &sn, &cs);
+    }
+    s_cos[warp][p] = cs;
+    s_sin[warp][p] = sn;
   }
   long long slot_off = 0, slot_hs = 0;  // element offset of head 0 of the token's slot in the pages
   bool stored = true;
@@ -159,41 +167,31 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 4) qk_norm_rope_kernel(const 
     slot_hs = static_cast<long long>(a.page_tokens) * D;
   }
   __syncwarp();
-  // half-split: pairs % 8 == 0, a lane's 8 dims are all first halves, all second halves or none
-  const int hl = pairs / 8;  // lanes of one half
-  const int side = INTERLEAVED ? 0 : j < hl ? -1 : j < 2 * hl ? 1 : 0;
-  const int partner = lane - side * hl;
+  const bool turns_here = INTERLEAVED || j < turning;
 
   auto pass = [&](const T* src, long long hs, T* dst, long long dst_hs, int heads, const float* weight, bool keep,
                   bool asked) {
     uint64_t fa[4], fb[4];
     {
-      float w[8], wo[8];  // of this lane's elements, of their partners
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = wo[i] = 1.0f;
+      float4 w0 = make_float4(1.0f, 1.0f, 1.0f, 1.0f), w1 = w0, c = w0, s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (NORM && weight) {
-        const float4* p = reinterpret_cast<const float4*>(weight + j * 8);
-        const float4* o = reinterpret_cast<const float4*>(weight + (j - side * hl) * 8);
-        const float4 x = p[0], y = p[1], z = o[0], v = o[1];
-        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w, w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
-        wo[0] = z.x, wo[1] = z.y, wo[2] = z.z, wo[3] = z.w, wo[4] = v.x, wo[5] = v.y, wo[6] = v.z, wo[7] = v.w;
+        w0 = *reinterpret_cast<const float4*>(weight + first);
+        w1 = *reinterpret_cast<const float4*>(weight + first + second);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (INTERLEAVED) {
-          const int p = 4 * j + i;
-          const float2 c = p < pairs ? s_cs[warp][p] : make_float2(1.0f, 0.0f);
-          fa[i] = pair_f32(w[2 * i] * c.x, w[2 * i + 1] * c.x);
-          fb[i] = pair_f32(-w[2 * i + 1] * c.y, w[2 * i] * c.y);
-        } else {
-          float2 c = make_float2(1.0f, 0.0f), d = c;
-          if (side) {
-            c = s_cs[warp][(side < 0 ? j : j - hl) * 8 + 2 * i];
-            d = s_cs[warp][(side < 0 ? j : j - hl) * 8 + 2 * i + 1];
-          }
-          fa[i] = pair_f32(w[2 * i] * c.x, w[2 * i + 1] * d.x);
-          fb[i] = pair_f32(side * wo[2 * i] * c.y, side * wo[2 * i + 1] * d.y);  // a cos - b sin, b cos + a sin
-        }
+      if (turns_here) {
+        c = *reinterpret_cast<const float4*>(&s_cos[warp][4 * j]);
+        s = *reinterpret_cast<const float4*>(&s_sin[warp][4 * j]);
+      }
+      if (INTERLEAVED) {  // pairs (0, 1) (2, 3) ..: a cos - b sin, b cos + a sin
+        fa[0] = pair_f32(w0.x * c.x, w0.y * c.x), fb[0] = pair_f32(-w0.y * s.x, w0.x * s.x);
+        fa[1] = pair_f32(w0.z * c.y, w0.w * c.y), fb[1] = pair_f32(-w0.w * s.y, w0.z * s.y);
+        fa[2] = pair_f32(w1.x * c.z, w1.y * c.z), fb[2] = pair_f32(-w1.y * s.z, w1.x * s.z);
+        fa[3] = pair_f32(w1.z * c.w, w1.w * c.w), fb[3] = pair_f32(-w1.w * s.w, w1.z * s.w);
+      } else {  // pairs (0, 4) (1, 5) ..
+        fa[0] = pair_f32(w0.x * c.x, w0.y * c.y), fa[1] = pair_f32(w0.z * c.z, w0.w * c.w);
+        fa[2] = pair_f32(w1.x * c.x, w1.y * c.y), fa[3] = pair_f32(w1.z * c.z, w1.w * c.w);
+        fb[0] = pair_f32(-w1.x * s.x, -w1.y * s.y), fb[1] = pair_f32(-w1.z * s.z, -w1.w * s.w);
+        fb[2] = pair_f32(w0.x * s.x, w0.y * s.y), fb[3] = pair_f32(w0.z * s.z, w0.w * s.w);
       }
     }
     for (int g0 = part; g0 * HPI < heads; g0 += U * wpt) {
@@ -202,11 +200,14 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 4) qk_norm_rope_kernel(const 
       for (int u = 0; u < U; ++u) {
         const int r0 = (g0 + u * wpt) * HPI, r = r0 + sub;
         if (r0 >= heads) break;  // warp-uniform
-        uint64_t scale = pair_f32(1.0f, 1.0f);
+        uint64_t x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = in[u].pair(i);
+        uint64_t scale = 0;
         if (NORM) {
           uint64_t sq = 0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sq = fma_f32x2(in[u].pair(i), in[u].pair(i), sq);
+          for (int i = 0; i < 4; ++i) sq = fma_f32x2(x[i], x[i], sq);
           const float2 s2 = unpair_f32(sq);
           float ss = s2.x + s2.y;
 #pragma unroll
@@ -215,40 +216,33 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 4) qk_norm_rope_kernel(const 
           scale = pair_f32(rs, rs);
         }
         Vec8<T> out;
-        if (INTERLEAVED) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint64_t x = in[u].pair(i);
-            const float2 f = unpair_f32(x);
-            uint64_t y = mul_f32x2(x, fa[i]);
+        for (int i = 0; i < 4; ++i) {
+          uint64_t y = mul_f32x2(x[i], fa[i]);
+          if (INTERLEAVED) {
+            const float2 f = unpair_f32(x[i]);
             if (4 * j + i < pairs) y = fma_f32x2(pair_f32(f.y, f.x), fb[i], y);
-            out.set(i, NORM ? mul_f32x2(y, scale) : y);
+          } else if (turns_here) {
+            y = fma_f32x2(x[i ^ 2], fb[i], y);
           }
-        } else {
-          const Vec8<T> other = in[u].of_lane(partner);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint64_t y = mul_f32x2(in[u].pair(i), fa[i]);
-            if (side) y = fma_f32x2(other.pair(i), fb[i], y);
-            out.set(i, NORM ? mul_f32x2(y, scale) : y);
-          }
+          out.set(i, NORM ? mul_f32x2(y, scale) : y);
         }
-        if (r < heads && keep) out.store(dst + r * dst_hs);
+        if (r < heads && keep) out.template store<TWO>(dst + r * dst_hs, second);
       }
     }
   };
-  pass(qp, a.q_hs, static_cast<T*>(a.q_out) + t * a.qo_ts + j * 8, a.qo_hs, a.heads, a.qw, true, true);
-  pass(kp, a.k_hs, static_cast<T*>(a.k_out) + (a.slots ? slot_off : t * a.ko_ts) + j * 8, a.slots ? slot_hs : a.ko_hs,
+  pass(qp, a.q_hs, static_cast<T*>(a.q_out) + t * a.qo_ts + first, a.qo_hs, a.heads, a.qw, true, true);
+  pass(kp, a.k_hs, static_cast<T*>(a.k_out) + (a.slots ? slot_off : t * a.ko_ts) + first, a.slots ? slot_hs : a.ko_hs,
        a.kv_heads, a.kw, stored, false);
   if (a.slots && stored) {
-    const T* vp = static_cast<const T*>(a.v) + t * a.v_ts + j * 8;
-    T* vo = static_cast<T*>(a.v_out) + slot_off + j * 8;
+    const T* vp = static_cast<const T*>(a.v) + t * a.v_ts + first;
+    T* vo = static_cast<T*>(a.v_out) + slot_off + first;
     for (int g0 = part; g0 * HPI < a.kv_heads; g0 += U * wpt) {
       ask(vp, a.v_hs, a.kv_heads, g0);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int r = (g0 + u * wpt) * HPI + sub;
-        if (r < a.kv_heads) in[u].store(vo + r * slot_hs);
+        if (r < a.kv_heads) in[u].template store<TWO>(vo + r * slot_hs, second);
       }
     }
   }
