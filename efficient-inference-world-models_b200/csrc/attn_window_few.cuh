@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, D == 64 ? (NR == 8 ? 4 : 3) : 
       m[t] = -INFINITY;
       l[t] = 0.0f;
     }
-    bool dirty = false;
+    uint32_t dirty = 0;
 
     // this warp's run of steps
     const int part = split * kFewWarps + warp, parts = splits * kFewWarps;
@@ -191,12 +191,14 @@ __global__ void __launch_bounds__(kFewWarps * 32, D == 64 ? (NR == 8 ? 4 : 3) : 
           // only some of the rows see has the rows computed one by one
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const bool seen = span.sees(key0 + 2 * c + (x & 1) + 8 * (x >> 1));
+            const int key = key0 + 2 * c + (x & 1) + 8 * (x >> 1);
+            if (span.all(key, key + 1)) continue;
+            const bool seen = span.sees(key);
 #pragma unroll
             for (int i = 0; i < VC; ++i) {
               if (!seen) vb[x][i] = make_uint4(0, 0, 0, 0);
-              dirty = dirty || nonfinite2<T>(vb[x][i].x) || nonfinite2<T>(vb[x][i].y) ||
-                      nonfinite2<T>(vb[x][i].z) || nonfinite2<T>(vb[x][i].w);
+              dirty |= nonfinite2<T>(vb[x][i].x) | nonfinite2<T>(vb[x][i].y) | nonfinite2<T>(vb[x][i].z) |
+                       nonfinite2<T>(vb[x][i].w);
             }
           }
         }

@@ -156,11 +156,12 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Whether one of the two 16-bit values of a word is an infinity or NaN.
+// Non-zero if one of the two 16-bit values of a word is an infinity or NaN: its magnitude is at least
+// that of infinity, and then what is missing to 2^15 carries into the sign bit.
 template <typename T>
-__device__ __forceinline__ bool nonfinite2(uint32_t w) {
-  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
-  return (w & e) == e || (w & (e << 16)) == (e << 16);
+__device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
+  constexpr uint32_t gap = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+  return ((w & 0x7FFF7FFFu) + gap) & 0x80008000u;
 }
 
 // Instruction descriptor of kind::f16 for this type: fp32 D, A K-major, B K-major or (b_mn) MN-major.
@@ -331,18 +332,26 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         if (!span.all(k0, k0 + kWtKeys)) {
           ok = __all_sync(0xffffffffu, mbar_wait(&full[st], (j / kSV) & 1));
           uint8_t* v = ring + st * S::kTile;
-          bool bad = false;
-          for (int r = lane / 8; ok && r < kWtKeys; r += 4) {
-            const bool seen = span.sees(k0 + r);
+          uint32_t bad = 0;
+#pragma unroll 1
+          for (int r0 = 0; ok && r0 < kWtKeys; r0 += 32) {
+            if (span.all(k0 + r0, k0 + r0 + 32)) continue;
 #pragma unroll
             for (int h = 0; h < D / 64; ++h) {
-              uint4* p = reinterpret_cast<uint4*>(v + h * S::kHalf + r * 128 + (lane % 8) * 16);
-              if (seen) {
-                const uint4 x = *p;
-                bad |= nonfinite2<T>(x.x) || nonfinite2<T>(x.y) || nonfinite2<T>(x.z) || nonfinite2<T>(x.w);
-              } else {
-                *p = make_uint4(0, 0, 0, 0);
+              uint4 x[8];  // 4 rows at a time, 8 loads in flight
+#pragma unroll
+              for (int u = 0; u < 8; ++u) {
+                const int r = r0 + u * 4 + lane / 8;
+                uint4* p = reinterpret_cast<uint4*>(v + h * S::kHalf + r * 128 + (lane % 8) * 16);
+                x[u] = make_uint4(0, 0, 0, 0);
+                if (!span.sees(k0 + r))
+                  *p = x[u];
+                else if (!span.all(k0 + r, k0 + r + 1))
+                  x[u] = *p;
               }
+#pragma unroll
+              for (int u = 0; u < 8; ++u)
+                bad |= nonfinite2<T>(x[u].x) | nonfinite2<T>(x[u].y) | nonfinite2<T>(x[u].z) | nonfinite2<T>(x[u].w);
             }
           }
           if (bad) *dirty = 1;
