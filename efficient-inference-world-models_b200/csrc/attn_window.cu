@@ -157,15 +157,21 @@ __device__ __noinline__ void window_row(const WinArgs& a, int b, const WinSeq& s
 
 namespace oasis {
 
-// Dynamic shared memory of a kernel above 48 KB, set once per device.
+// Dynamic shared memory of a kernel above 48 KB, set once per device; `registers`: per thread, checked.
 template <auto Kernel>
-int allow_smem(int bytes, const char* what) {
+int allow_smem(int bytes, int registers, const char* what) {
   static std::atomic<uint64_t> done{0};  // one per kernel
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e, what);
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (bit && (done.load(std::memory_order_acquire) & bit)) return OASIS_OK;
+  if (registers) {  // what the kernel shares out anew is what the block starts with, or it waits for good
+    cudaFuncAttributes attr;
+    e = cudaFuncGetAttributes(&attr, Kernel);
+    if (e != cudaSuccess) return cuda_status(e, what);
+    if (attr.numRegs != registers) return fail(OASIS_ERR_UNSUPPORTED, std::string(what) + ": built with other registers");
+  }
   e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return cuda_status(e, what);
   done.fetch_or(bit, std::memory_order_release);
@@ -241,18 +247,45 @@ int tile_splits(long long pairs, long long keys) {
   return best;
 }
 
-template <typename T, int D, int NR>
-int launch_attn_window_few(const WinArgs& a, int max_kv, cudaStream_t stream) {
-  // CTAs per (sequence, key head): six per SM, where three (D = 128) are resident at a time, so that
-  // ragged sequences even out; a warp keeps a step of 16 keys at least.  32 ragged sequences of 8 key
-  // heads: 151 us with 4, 164 with 2 or 8, 187 with 1.
-  const long long base = static_cast<long long>(a.batch) * a.kv_heads;
-  const long long steps = (visible_keys(a, max_kv) + 15) / 16;
-  const long long want = (6LL * num_sms() + base - 1) / base;
-  const int splits = static_cast<int>(std::max(1LL, std::min({want, (steps + kFewWarps - 1) / kFewWarps,
-                                                              static_cast<long long>(kWinSplits)})));
-  cudaError_t e = launch_pdl_cluster(attn_window_few_kernel<T, D, NR>, dim3(splits * a.kv_heads, 1, a.batch),
-                                     dim3(kFewWarps * 32), 0, stream, splits, a, splits);
+// Whether the device takes clusters of kFewSplits CTAs of this kernel (more than the portable 8), asked
+// once per device.
+template <auto Kernel, int Threads>
+bool wide_clusters() {
+  static std::atomic<int> known[64];  // 1: no, 2: yes
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return false;
+  if (const int k = known[dev].load(std::memory_order_acquire)) return k == 2;
+  int n = 0;
+  bool fine = cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
+  if (fine) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kFewSplits);
+    cfg.blockDim = dim3(Threads);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kFewSplits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    fine = cudaOccupancyMaxActiveClusters(&n, Kernel, &cfg) == cudaSuccess && n > 0;
+  }
+  if (!fine) (void)cudaGetLastError();
+  known[dev].store(fine ? 2 : 1, std::memory_order_release);
+  return fine;
+}
+
+template <typename T, int D, int NR, int NW>
+int launch_attn_window_few(const WinArgs& a, long long base, long long steps, cudaStream_t stream) {
+  // CTAs per (sequence, key head): six of 4 warps per SM, where three (D = 128) are resident at a time,
+  // so that ragged sequences even out; a warp keeps a step of 16 keys at least.  32 ragged sequences of
+  // 8 key heads: 151 us with 4, 164 with 2 or 8, 187 with 1.
+  const long long want = std::min((6LL * num_sms() + base - 1) / base, (steps + NW - 1) / NW);
+  constexpr auto kernel = attn_window_few_kernel<T, D, NR, NW>;
+  const bool more = want > kWinSplits && base * kWinSplits * NW <= 256 && wide_clusters<kernel, NW * 32>();
+  const long long most = more ? kFewSplits : kWinSplits;
+  const int splits = static_cast<int>(std::max(1LL, std::min(want, most)));
+  cudaError_t e = launch_pdl_cluster(kernel, dim3(splits * a.kv_heads, 1, a.batch), dim3(NW * 32), 0, stream, splits, a,
+                                     splits);
   if (e != cudaSuccess) return cuda_status(e, "attn_window_few_kernel");
   return OASIS_OK;
 }
@@ -265,7 +298,7 @@ int launch_attn_window(const WinArgs& a, int max_q, int max_kv, cudaStream_t str
     CUtensorMap tk, tv;
     if (int st = encode_page_rows(&tk, a.k, a, D, box)) return st;
     if (int st = encode_page_rows(&tv, a.v, a, D, box)) return st;
-    if (int st = allow_smem<attn_window_tile_kernel<T, D>>(WtShape<D>::kSmem, "attn_window_tile_kernel")) return st;
+    if (int st = allow_smem<attn_window_tile_kernel<T, D>>(WtShape<D>::kSmem, kWtRegs, "attn_window_tile_kernel")) return st;
     const int row_tiles = static_cast<int>((max_rows + 2 * kWtRows - 1) / (2 * kWtRows));
     const int splits = tile_splits<T, D>(static_cast<long long>(row_tiles) * a.kv_heads * a.batch, visible_keys(a, max_kv));
     if (static_cast<long long>(row_tiles) * a.kv_heads * splits > 0x7fffffffLL)
@@ -276,8 +309,18 @@ int launch_attn_window(const WinArgs& a, int max_q, int max_kv, cudaStream_t str
     if (e != cudaSuccess) return cuda_status(e, "attn_window_tile_kernel");
     return OASIS_OK;
   }
-  return max_rows <= 8 ? launch_attn_window_few<T, D, 8>(a, max_kv, stream)
-                       : launch_attn_window_few<T, D, 16>(a, max_kv, stream);
+  // Few pairs of a sequence and a key head: twice the warps per CTA (1 sequence of 16,000 tokens and 8 key
+  // heads of 128: 22 us against 35), and clusters of up to 16 where those would still leave most SMs
+  // without work (1 key head: 13 us against 20; with 8 key heads they take 26, clusters of 16 lying worse).
+  const long long base = static_cast<long long>(a.batch) * a.kv_heads;
+  const long long steps = (visible_keys(a, max_kv) + 15) / 16;
+  const bool wide = base * 64 <= 12LL * num_sms() && steps >= 4 * kWinSplits;
+  if (max_rows <= 8)
+    return wide ? launch_attn_window_few<T, D, 8, 8>(a, base, steps, stream)
+                : launch_attn_window_few<T, D, 8, 4>(a, base, steps, stream);
+  if constexpr (D == 64)  // (the parts of 8 warps, 16 rows and 128 dims would not fit)
+    if (wide) return launch_attn_window_few<T, D, 16, 8>(a, base, steps, stream);
+  return launch_attn_window_few<T, D, 16, 4>(a, base, steps, stream);
 }
 
 }  // namespace oasis

@@ -9,13 +9,13 @@
 //                supplies 16-byte chunks c, c + 4, ... of its key, and Q takes the same order of dims;
 //   O^T = V^T P^T  P's accumulators are the B operand as they stand; thread (g, c) supplies keys
 //                2c, 2c+1, 2c+8, 2c+9 and dims 8g .. 8g+7 (+64), paired by byte permutes.
-// The warps of a CTA, then the CTAs of a cluster (up to 8, over distributed shared memory), join their
-// maxima, sums and O in a fixed order: no workspace and no second launch.
+// The warps of a CTA (NW), then the CTAs of a cluster (up to 16, over distributed shared memory), join
+// their maxima, sums and O in a fixed order: no workspace and no second launch.
 #pragma once
 
 namespace oasis {
 
-constexpr int kFewWarps = 4;
+constexpr int kFewSplits = 16;  // CTAs of a cluster, at most (above 8: where the device takes such clusters)
 
 template <typename T>
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -41,25 +41,25 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
   return v;
 }
 
-template <int D, int NR>
+template <int D, int NR, int NW>
 struct alignas(16) FewShared {
-  float o[kFewWarps][NR][D];
-  float m[kFewWarps][NR], l[kFewWarps][NR];
+  float o[NW][NR][D];
+  float m[NW][NR], l[NW][NR];
   // from the CTAs of the cluster: maxima and sums of all rows, and of this CTA's share of O, 4 dims
   // of a row at a time, unit e of the whole in place e / CTAs of CTA e % CTAs
-  float cm[kWinSplits][NR], cl[kWinSplits][NR];
-  float4 co[NR * D / 4 + kWinSplits];
-  uint32_t marks[kWinSplits];
+  float cm[kFewSplits][NR], cl[kFewSplits][NR];
+  float4 co[NR * D / 4 + kFewSplits];
+  uint32_t marks[kFewSplits];
   uint32_t dirty;
 };
 
-template <typename T, int D, int NR>
-__global__ void __launch_bounds__(kFewWarps * 32, D == 64 ? (NR == 8 ? 4 : 3) : (NR == 8 ? 3 : 2))
+template <typename T, int D, int NR, int NW>
+__global__ void __launch_bounds__(NW * 32, NW == 8 ? 1 : D == 64 ? (NR == 8 ? 4 : 3) : (NR == 8 ? 3 : 2))
     attn_window_few_kernel(const __grid_constant__ WinArgs a, int splits) {
   constexpr int KC = D / 32;  // 16-byte chunks of a key per thread
   constexpr int VC = D / 64;  // of a value
   constexpr int RT = NR / 8;
-  __shared__ FewShared<D, NR> sh;
+  __shared__ FewShared<D, NR, NW> sh;
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, D == 64 ? (NR == 8 ? 4 : 3) : 
     uint32_t dirty = 0;
 
     // this warp's run of steps
-    const int part = split * kFewWarps + warp, parts = splits * kFewWarps;
+    const int part = split * NW + warp, parts = splits * NW;
     const int j0 = static_cast<int>(static_cast<long long>(steps.n) * part / parts);
     const int j1 = static_cast<int>(static_cast<long long>(steps.n) * (part + 1) / parts);
     uint4 kb[2][KC], vb[4][VC];
@@ -294,15 +294,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, D == 64 ? (NR == 8 ? 4 : 3) : 
     // what the others may write to: the CTAs are all here, and done with an earlier turn's parts
     if (splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     const int units = (row1 - row0) * (D / 4), share = (units + splits - 1) / splits;
-    for (int e = threadIdx.x; e < units; e += kFewWarps * 32) {
+    for (int e = threadIdx.x; e < units; e += NW * 32) {
       const int r = e / (D / 4), d = (e % (D / 4)) * 4;
       float top = sh.m[0][r];
 #pragma unroll
-      for (int w = 1; w < kFewWarps; ++w) top = join_max(top, sh.m[w][r]);
+      for (int w = 1; w < NW; ++w) top = join_max(top, sh.m[w][r]);
       float sum = 0.0f;
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int w = 0; w < kFewWarps; ++w) {
+      for (int w = 0; w < NW; ++w) {
         const float f = weight(sh.m[w][r], top);
         const float4 x = *reinterpret_cast<const float4*>(&sh.o[w][r][d]);
         sum += f * sh.l[w][r];
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, D == 64 ? (NR == 8 ? 4 : 3) : 
       for (int r = row0 + part; r < row1; r += parts)
         window_row<T, D>(a, b, seq, a.by_group.div(r), kvh * a.group + a.by_group.mod(r), lane);
     } else {
-      for (int i = threadIdx.x; i * splits + split < units; i += kFewWarps * 32) {
+      for (int i = threadIdx.x; i * splits + split < units; i += NW * 32) {
         const int e = i * splits + split;
         const int r = e / (D / 4), d = (e % (D / 4)) * 4;
         float top = -INFINITY;

@@ -4,8 +4,8 @@
 // Rows are the queries of the key head's group, token-major (row r: token r / group, head
 // r % group), so grouped heads share every key tile.  A CTA holds two tiles of 128 rows.
 // Roles: warps 0-3 and 4-7 are the softmax of tile 0 and 1 (one row per thread, S read from
-// TMEM); warp 8 issues the MMAs; warp 9 loads K and V tiles of 128 keys page by page and looks
-// over the V tiles that some row sees only in part.
+// TMEM); warp 8 issues the MMAs; warps 9 and 10 load K and V tiles of 128 keys page by page;
+// warp 11 looks over the V tiles that some row sees only in part.
 //
 // For tile i and key tile j:  S_i = Q_i K_j^T (TMEM, 128 columns), the softmax thread takes
 // P = exp2(S * scale - m) and writes it in 16 bits over S, O_i += P_i V_j (P from TMEM).  The MMA warp
@@ -19,7 +19,8 @@ namespace oasis {
 
 constexpr int kWtRows = 128;     // query rows of a tile
 constexpr int kWtKeys = 128;     // keys of a K/V tile
-constexpr int kWtThreads = 320;  // 8 softmax warps, MMA, loads: 200 registers each
+constexpr int kWtThreads = 384;  // 8 softmax warps, MMA, K loads, V loads, V looked over
+constexpr int kWtRegs = 168;     // per thread at launch (which checks it); the softmax warps take from the others
 constexpr float kWtLazy = 8.0f;  // log2 of how far scores may pass the maximum in use
 
 template <int D>
@@ -32,9 +33,13 @@ struct WtShape {
   static constexpr int kBars = 3 * kStages + 12;
   // D = 64 leaves TMEM columns for P beside S: the next S is then computed under the softmax
   static constexpr bool kEarly = D == 64;
-  // quarters of P that the MMAs get before the rest is there: 416 us with two against 423 with three
-  // for a prompt of 8,191 tokens at D = 128, 75 against 71 us for 8 sessions' frames at D = 64
+  // quarters of P that the MMAs get before the rest is there: two or three, 384 or 399 us for a prompt of
+  // 8,191 tokens at D = 128, 77.4 or 76.7 us for 8 sessions' frames at D = 64 (with 200 registers)
   static constexpr int kHandover = kEarly ? 3 : 2;
+  // registers of a softmax and of a helping thread: the prompt takes 390 us with 208 and 88, 8 sessions'
+  // frames 80 (the compiler orders the softmax by what it has)
+  static constexpr int kSoftRegs = D == 128 ? 200 : 216, kHelpRegs = D == 128 ? 104 : 72;
+  static_assert(256 * kSoftRegs + 128 * kHelpRegs <= kWtThreads * kWtRegs, "registers of the block");
   static constexpr int kO = 256, kP = kEarly ? kO + 2 * D : 0, kPStep = kEarly ? 64 : 128;  // columns of tile 0, 1
   static constexpr int kSmem = (2 + kStages) * kTile + 1024 + 256 + 8 * kBars;
 };
@@ -49,6 +54,12 @@ __device__ __forceinline__ uint64_t wt_v_desc(uint32_t smem_addr) {
   d |= static_cast<uint64_t>(2u) << 61;  // SWIZZLE_128B
   return d;
 }
+
+// Register shares within a block (WtShape).
+template <int N>
+__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // D (+)= A B^T with A from shared memory, and with A (P, K-major) from TMEM.
 __device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
@@ -285,7 +296,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
   const int n = tiles.n;
   // The parts that the CTAs of a cluster send each other, over the ring once all are done with it:
   // of every CTA, for this one's share of the rows, O [share][D] fp32 (16-byte chunks swizzled by
-  // row), the rows' maxima and sums, and the mark of warp 9.
+  // row), the rows' maxima and sums, and the mark of warp 11.
   const int share = (row1 - row0 + splits - 1) / splits;
   float* part_o = reinterpret_cast<float*>(ring);
   float* part_m = part_o + splits * share * D;
@@ -298,14 +309,13 @@ __global__ void __launch_bounds__(kWtThreads, 1)
   bool ok = true;
 
   if (warp >= 8) {
+    reg_dec<S::kHelpRegs>();
     if (row0 >= rows) {
       // nothing to do
-    } else if (warp == 9) {
-      // -------------------------------------------------------------- loads, and V tiles seen in part
-      // A V tile that some query does not see whole is looked over before the MMAs may have it:
-      // rows that no query of this CTA sees (ends of pages, tokens before the window) are zeroed, since
-      // their weights are 0 but 0 * NaN is not; an infinity or NaN in a row that only some queries
-      // see marks the CTA, whose rows are then computed one by one (window_row).
+    } else if (warp == 9 || warp == 10) {
+      // -------------------------------------------------------------- loads: warp 9 K, warp 10 V
+      const bool is_k = warp == 9;
+      const int ring0 = is_k ? 0 : kSK, slots = is_k ? kSK : kSV;
       const int boxes = kWtKeys / box_rows;
       const int none = a.pages * a.kv_heads * a.page_tokens;  // beyond the pages: zeros
       auto box_row = [&](int j) {  // lane x takes box x
@@ -315,26 +325,50 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         return page >= 0 && page < a.pages ? (page * a.kv_heads + kvh) * a.page_tokens + (key - idx * a.page_tokens)
                                            : none;
       };
-      auto load = [&](const CUtensorMap& map, int slot, int row) {
+      auto load = [&](int j, int row) {
+        const int slot = ring0 + j % slots;
         if (lane == 0) mbar_arrive_expect_tx(&full[slot], S::kTile);
         __syncwarp();
         if (lane < boxes) {
+          uint8_t* dst = ring + slot * S::kTile + lane * box_rows * 128;
+          // (two calls: a selected pointer would make the compiler copy the maps to the stack)
 #pragma unroll
-          for (int h = 0; h < D / 64; ++h)
-            tma_load_2d(ring + slot * S::kTile + lane * box_rows * 128 + h * S::kHalf, &map, &full[slot], h * 64, row);
+          for (int h = 0; h < D / 64; ++h) {
+            if (is_k)
+              tma_load_2d(dst + h * S::kHalf, &tm_k, &full[slot], h * 64, row);
+            else
+              tma_load_2d(dst + h * S::kHalf, &tm_v, &full[slot], h * 64, row);
+          }
         }
         __syncwarp();
       };
-      auto look_over = [&](int j) {
+      bool ok = true;
+      int j = 0, row = n > 0 ? box_row(0) : none;
+      for (; j < n; ++j) {
+        const int next = j + 1 < n ? box_row(j + 1) : none;  // looked up under the wait
+        if (j >= slots) ok = __all_sync(0xffffffffu, mbar_wait(&empty[ring0 + j % slots], (j / slots - 1) & 1));
+        if (!ok) break;
+        load(j, row);
+        row = next;
+      }
+      if (!ok)  // gave up: let the copies in flight land before the memory is given back
+        for (int i = max(0, j - slots); i < j; ++i) mbar_wait(&full[ring0 + i % slots], (i / slots) & 1);
+    } else if (warp == 11) {
+      // -------------------------------------------------------------- V tiles seen in part
+      // A V tile that some query does not see whole is looked over before the MMAs may have it:
+      // rows that no query of this CTA sees (ends of pages, tokens before the window) are zeroed, since
+      // their weights are 0 but 0 * NaN is not; an infinity or NaN in a row that only some queries
+      // see marks the CTA, whose rows are then computed one by one (window_row).
+      bool ok = true;
+      for (int j = 0; j < n && ok; ++j) {
         const int st = kSK + j % kSV;
         const int k0 = tiles.tile(j) * kWtKeys;
-        bool ok = true;
-        if (!span.all(k0, k0 + kWtKeys)) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&full[st], (j / kSV) & 1));
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[st], (j / kSV) & 1));
+        if (ok && !span.all(k0, k0 + kWtKeys)) {
           uint8_t* v = ring + st * S::kTile;
           uint32_t bad = 0;
 #pragma unroll 1
-          for (int r0 = 0; ok && r0 < kWtKeys; r0 += 32) {
+          for (int r0 = 0; r0 < kWtKeys; r0 += 32) {
             if (span.all(k0 + r0, k0 + r0 + 32)) continue;
 #pragma unroll
             for (int h = 0; h < D / 64; ++h) {
@@ -359,35 +393,6 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&clean[st]);
-        return ok;
-      };
-      int nk = 0, nv = 0;  // tiles asked for
-      constexpr int kFirst = kSK > kSV ? kSK : kSV;
-      int rows_of[kFirst];  // the look-ups of the first tiles run side by side
-#pragma unroll
-      for (int j = 0; j < kFirst; ++j) rows_of[j] = j < n ? box_row(j) : none;
-#pragma unroll
-      for (int j = 0; j < kFirst; ++j) {
-        if (j < min(n, kSK)) load(tm_k, nk++, rows_of[j]);
-        if (j < min(n, kSV)) load(tm_v, kSK + nv++, rows_of[j]);
-      }
-      bool ok = n == 0 || look_over(0);
-      for (int j = 0; j < n && ok; ++j) {
-        if (nk < n) {
-          const int row = box_row(nk);
-          ok = __all_sync(0xffffffffu, mbar_wait(&empty[j % kSK], (j / kSK) & 1));
-          if (ok) load(tm_k, nk++ % kSK, row);
-        }
-        if (ok && j + 1 < n) ok = look_over(j + 1);
-        if (ok && nv < n) {
-          const int row = box_row(nv);
-          ok = __all_sync(0xffffffffu, mbar_wait(&empty[kSK + j % kSV], (j / kSV) & 1));
-          if (ok) load(tm_v, kSK + nv++ % kSV, row);
-        }
-      }
-      if (!ok) {  // gave up: let the copies in flight land before the memory is given back
-        for (int j = max(0, nk - kSK); j < nk; ++j) mbar_wait(&full[j % kSK], (j / kSK) & 1);
-        for (int j = max(0, nv - kSV); j < nv; ++j) mbar_wait(&full[kSK + j % kSV], (j / kSV) & 1);
       }
     } else {
       // -------------------------------------------------------------- MMA: one lane issues, the
@@ -521,6 +526,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       }
     }
   } else {
+    reg_inc<S::kSoftRegs>();
     if (row0 < rows) {
       // -------------------------------------------------------------- softmax
       const int i = warp >> 2;                  // tile
@@ -649,37 +655,18 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         const float base = m == -INFINITY ? 0.0f : fmaf(m, 0.0f, -m * sl2);  // NaN for a maximum of +inf
         uint64_t sum[2] = {0, 0};
         // (D = 128: the columns of P lie over those of S, which are all in registers.)  The MMAs take
-        // the first kHandover quarters of the keys while the rest is computed.  The order in which the
-        // source has a quarter's arithmetic is the order in which it is issued: pair by pair at D = 64
-        // (8 sessions' frames 68 us, 74 in sweeps), in three sweeps at D = 128 (the prompt 416, 433 by pairs).
+        // the first kHandover quarters of the keys while the rest is computed.
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
-          if (S::kEarly) {
 #pragma unroll
-            for (int x = 0; x < 32; x += 2) {
-              float2 e =
-                  unpair_f32(fma_f32x2(pair_f32(v[c][x], v[c][x + 1]), pair_f32(sl2, sl2), pair_f32(base, base)));
-              e.x = ex2(e.x);
-              e.y = ex2(e.y);
-              sum[(x >> 1) & 1] = add_f32x2(sum[(x >> 1) & 1], pair_f32(e.x, e.y));
-              pk[x / 2] = pack2<T>(e.x, e.y);
-            }
-          } else {
-#pragma unroll
-            for (int x = 0; x < 32; x += 2) {
-              const float2 t =
-                  unpair_f32(fma_f32x2(pair_f32(v[c][x], v[c][x + 1]), pair_f32(sl2, sl2), pair_f32(base, base)));
-              v[c][x] = __float_as_uint(t.x);
-              v[c][x + 1] = __float_as_uint(t.y);
-            }
-#pragma unroll
-            for (int x = 0; x < 32; ++x) v[c][x] = __float_as_uint(ex2(__uint_as_float(v[c][x])));
-#pragma unroll
-            for (int x = 0; x < 32; x += 2) {
-              sum[(x >> 1) & 1] = add_f32x2(sum[(x >> 1) & 1], pair_f32(v[c][x], v[c][x + 1]));
-              pk[x / 2] = pack2<T>(__uint_as_float(v[c][x]), __uint_as_float(v[c][x + 1]));
-            }
+          for (int x = 0; x < 32; x += 2) {
+            float2 e =
+                unpair_f32(fma_f32x2(pair_f32(v[c][x], v[c][x + 1]), pair_f32(sl2, sl2), pair_f32(base, base)));
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            sum[(x >> 1) & 1] = add_f32x2(sum[(x >> 1) & 1], pair_f32(e.x, e.y));
+            pk[x / 2] = pack2<T>(e.x, e.y);
           }
           if (c == S::kHandover) {
             tmem_wait_st(pk);  // of the earlier quarters, under the arithmetic of this one
@@ -700,7 +687,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       if (ok && np > 0) ok = mbar_wait(&pv_done[i], (np - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      // warp 9's mark: every tile it looked at was multiplied before pv_done
+      // warp 11's mark: every tile it looked at was multiplied before pv_done
       if (splits > 1) {
         // joined below
       } else if (ok && *reinterpret_cast<volatile uint32_t*>(dirty)) {

@@ -272,6 +272,10 @@ TOKEN = [  # single tokens and few rows
     ([7], [3], 2, 1, 64, BF, 16, None, 0, 1),                 # more queries than tokens: rows that see nothing
     ([2, 1], [0, 0], 4, 4, 64, HF, 16, 5, 1, 1),              # empty caches
     ([1, 1], [600, 500], 20, 1, 128, BF, 16, 99, 99, 3),      # 20 rows on one key head
+    ([1], [6001], 8, 1, 128, BF, 16, None, 0, 1),             # one key head: the widest splits
+    ([1], [5003], 16, 1, 128, HF, 32, 4000, 30, 1),
+    ([2], [4100], 16, 2, 64, BF, 16, 1000, 10, 1),
+    ([1, 1], [3000, 100], 24, 12, 128, BF, 48, None, 0, 1),
 ]
 
 TILE = [  # prompts and frames
@@ -310,6 +314,7 @@ def test_attn_window_page_holes(pkg, cuda, q_len):
     holes = [(0, 0, -1), (0, 5, 1 << 30), (0, 6, -(1 << 31)), (1, 3, -7), (1, 1, 99999)]
     run_case(pkg, cuda, q_len, [300, 170], 4, 2, 64, BF, 16, None, 0, 1, holes=holes)
     run_case(pkg, cuda, q_len, [300, 170], 4, 2, 128, HF, 16, 64, 20, 1, holes=holes)
+    run_case(pkg, cuda, q_len, [3000, 1700], 4, 2, 128, BF, 16, None, 0, 1, holes=holes)
 
 
 @pytest.mark.parametrize("q_len", [[1, 1], [3, 2], [150, 130]])
