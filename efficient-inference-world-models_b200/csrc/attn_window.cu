@@ -100,8 +100,11 @@ __device__ __forceinline__ void st_cluster4(uint32_t addr, uint32_t x, uint32_t 
   asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w)
                : "memory");
 }
+
 // One query row by one warp, key after key with the running maximum and sum: each lane holds
-// D / 32 dims.  Reads only what the row sees.
+// D / 32 dims.  Reads only what the row sees.  For the rows that the tiled kernels leave: those of a
+// launch that was told of fewer, and those of a CTA with infinities or NaN in values that only some of
+// its rows see.
 template <typename T, int D>
 __device__ __noinline__ void window_row(const WinArgs& a, int b, const WinSeq& s, int qi, int head, int lane) {
   constexpr int E = D / 32;
@@ -342,7 +345,7 @@ extern "C" int oasis_attn_window(const oasis_attn_window_t* p, cudaStream_t stre
     return fail(OASIS_ERR_UNSUPPORTED, std::string(who) + ": page_tokens must be a multiple of 16");
   if (p->dtype != OASIS_DT_BF16 && p->dtype != OASIS_DT_FP16)
     return fail(OASIS_ERR_UNSUPPORTED, std::string(who) + ": bf16 or fp16");
-  if (!(p->scale > 0.0f) || p->scale > 3.0e38f)
+  if (!(p->scale > 0.0f) || p->scale > 2.0e38f)
     return fail(OASIS_ERR_INVALID_ARG, std::string(who) + ": scale must be positive and finite");
   if (p->batch > 65535 || p->heads > 65535)
     return fail(OASIS_ERR_UNSUPPORTED, std::string(who) + ": at most 65535 sequences and heads");

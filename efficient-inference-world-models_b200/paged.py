@@ -323,7 +323,8 @@ def attn_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, p
     sees the frames up to its own that are fewer than ``window`` frames back (None: all) or among
     the first ``sinks``.  ``scale`` defaults to head_dim ** -0.5.  A query that sees nothing gets zeros.
 
-    ``max_q`` / ``max_kv`` (bounds on the queries and tokens of a sequence) only choose the launch.
+    ``max_q`` / ``max_kv`` (bounds on the queries and tokens of a sequence) only choose the launch; too
+    small ones cost time.
     Rows that belong to no sequence are not written.  ``out`` may be q.  Returns out, or (out, lse)
     with lse fp32 [tokens][heads], the natural logarithm of the softmax sum."""
     dev = q.get_device()

@@ -403,8 +403,9 @@ int oasis_qk_norm_rope(const oasis_qk_norm_rope_t* args, cudaStream_t stream);
  * logarithm.  Keys and values that a query does not see do not reach its result, whatever
  * they hold.
  * heads % kv_heads == 0; head_dim 64 or 128; page_tokens % 16 == 0; bf16 or fp16.
- * max_q and max_kv are bounds for choosing the launch (0: from the shapes); they do not
- * change the result. */
+ * kv_len is cut to what the table holds, cu_q to the rows there are.  max_q and max_kv are bounds
+ * for choosing the launch (0: from the shapes); they do not change the result, but bounds that
+ * are too small cost time. */
 typedef struct {
   const void* q; void* out; float* lse;
   long long q_token_stride, q_head_stride, out_token_stride, out_head_stride;
