@@ -451,6 +451,7 @@ class PagedBatchB200:
         self.max_q = 0
         self.seqs: Tuple[int, ...] = ()
         self.stale = True
+        self.cache: Optional[weakref.ref] = None  # whose pages it names
         n = 2 * sequences + 1 + sequences * width + tokens
         self._buffer = torch.empty(n, dtype=torch.int32, device=device)
         cu, lens, table, slots = self._buffer.split([sequences + 1, sequences, sequences * width, tokens])
@@ -547,10 +548,13 @@ class PagedKVCacheB200:
 
     def fork(self, seq: int, copies: int = 1) -> List[int]:
         """``copies`` new sessions that continue ``seq``: they share its pages, and whoever writes
-        into a shared page first gets a copy of it.  No device work."""
+        into a shared page first gets a copy of it.  No device work.  Plans that write into ``seq`` are
+        out of date from here on: their slots are shared now."""
         s = self._get(seq)
         if copies < 0:
             raise ValueError("copies must be >= 0")
+        if copies:
+            s.changed()
         for p in s.pages:
             if p >= 0:
                 self._refs[p] += copies
@@ -657,6 +661,8 @@ class PagedKVCacheB200:
         width = into.width if into is not None else max(need, table_width or 0)
         if need > width:
             raise ValueError(f"the plan has room for {width} pages per session, {need} are needed")
+        if into is not None and into.cache is not None and into.cache() is not self:
+            raise ValueError("the plan is of another cache")
         if into is not None and (into.sequences != len(seqs) or into.tokens != total):
             raise ValueError(f"the plan is for {into.sequences} sessions and {into.tokens} tokens")
         if width * pt > 0x3fffffff:
@@ -686,6 +692,7 @@ class PagedKVCacheB200:
         else:
             b._buffer.copy_(torch.from_numpy(host))
         b.max_q = max(max(counts), b.max_q)  # a captured launch keeps the bound it was captured with
+        b.cache = weakref.ref(self)
         for i in b.seqs:  # a rebuilt plan no longer follows its earlier sessions
             old = self._seqs.get(i)
             if old is not None:
@@ -731,6 +738,8 @@ class PagedKVCacheB200:
 
     # -- a layer's operators on a step -----------------------------------------------------
     def _live(self, batch: PagedBatchB200) -> None:
+        if batch.cache is None or batch.cache() is not self:
+            raise ValueError("the plan is of another cache")
         if batch.stale:
             raise ValueError("the step's plan is out of date: its sessions' pages have changed since")
 

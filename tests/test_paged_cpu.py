@@ -146,6 +146,24 @@ def test_plans_go_stale_and_are_rebuilt(pkg):
     assert s.stale
 
 
+def test_plans_of_forked_sessions_and_of_other_caches(pkg):
+    """A plan must not write into pages that a fork shares, nor be used on another cache."""
+    c, other = make(pkg), make(pkg)
+    a = c.new()
+    s = c.step([a], 3)
+    b = c.fork(a)[0]
+    z = torch.zeros(3, 2, 64)
+    with pytest.raises(ValueError, match="out of date"):
+        c.append(0, s, z, z, z, None, None, axes=(64,))
+    again = c.step([a], 3, extend=False)  # the same tokens, in a page of its own
+    assert c.pages_of(a) != c.pages_of(b) and not again.stale
+    owned(c)
+    n = other.new()
+    for call in (lambda: other.attend(0, again, z), lambda: other.step([n], 3, into=again)):
+        with pytest.raises(ValueError, match="another cache"):
+            call()
+
+
 @pytest.mark.parametrize("bad", ["twice", "none", "unknown", "negative", "few", "rewrite"])
 def test_step_refusals(pkg, bad):
     c = make(pkg)
