@@ -33,8 +33,8 @@ struct WtShape {
   static constexpr int kBars = 3 * kStages + 12;
   // D = 64 leaves TMEM columns for P beside S: the next S is then computed under the softmax
   static constexpr bool kEarly = D == 64;
-  // quarters of P that the MMAs get before the rest is there: two or three, 384 or 399 us for a prompt of
-  // 8,191 tokens at D = 128, 77.4 or 76.7 us for 8 sessions' frames at D = 64 (with 200 registers)
+  // quarters of P that the MMAs get before the rest is there: with two or three, 384 or 399 us for a
+  // prompt of 8,191 tokens at D = 128, 77 or 71 us for 8 sessions' frames at D = 64
   static constexpr int kHandover = kEarly ? 3 : 2;
   // registers of a softmax and of a helping thread: the prompt takes 390 us with 208 and 88, 8 sessions'
   // frames 80 (the compiler orders the softmax by what it has)

@@ -108,8 +108,8 @@ constexpr int kRopeWarps = 8;
 // Weight and rotation of a lane's elements become two factors each, kept for all heads of the
 // token:  y = rsqrt(mean) * (A x + B x'),  x' the other element of the pair.
 // Bound by HBM and by instructions at once: 36,864 tokens of 32 heads x 64 (302 MB) take
-// 57 us, 5.3 TB/s with 70 % of the issue slots busy (91 us with one fp32 shuffle per element of a
-// half-split pair and the factors unfolded).
+// 57 us, 5.3 TB/s with 70 % of the issue slots busy (63 us when the partners of the half-split pairs came by
+// shuffle; more warps per SM with fewer rows in flight 72, fewer with more rows 71).
 template <typename T, int D, bool INTERLEAVED, bool NORM>
 __global__ void __launch_bounds__(kRopeWarps * 32, 4) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int L = D / 8;
