@@ -459,13 +459,15 @@ class PagedBatchB200:
 
 
 class _Stream:
-    """Host record of a session: its pages in order (-1: evicted) and its tokens."""
+    """Host record of a session: its pages in order (-1: evicted), its tokens, and how far pages went
+    under each (window, sinks, frame_tokens) of its evictions (a page number, exclusive)."""
 
-    __slots__ = ("pages", "length", "batches")
+    __slots__ = ("pages", "length", "batches", "gone")
 
-    def __init__(self, pages: List[int], length: int):
+    def __init__(self, pages: List[int], length: int, gone: Optional[Dict[Tuple[int, int, int], int]] = None):
         self.pages, self.length = pages, length
         self.batches: List[weakref.ref] = []
+        self.gone = dict(gone or {})
 
     def changed(self) -> None:
         """The plans made of this record no longer describe it."""
@@ -558,7 +560,7 @@ class PagedKVCacheB200:
         for p in s.pages:
             if p >= 0:
                 self._refs[p] += copies
-        return [self._put(_Stream(list(s.pages), s.length)) for _ in range(copies)]
+        return [self._put(_Stream(list(s.pages), s.length, s.gone)) for _ in range(copies)]
 
     def free(self, seq: int) -> None:
         """End a session; pages that no other session shares become free."""
@@ -569,7 +571,8 @@ class PagedKVCacheB200:
         del self._seqs[seq]
 
     def truncate(self, seq: int, length: int) -> None:
-        """Keep the first ``length`` tokens (rejected frames go).  Evicted pages stay evicted."""
+        """Keep the first ``length`` tokens (rejected frames go).  Evicted pages stay evicted; a step whose
+        tokens see them is refused."""
         s = self._get(seq)
         if not 0 <= length <= s.length:
             raise ValueError(f"length must be 0..{s.length}")
@@ -577,25 +580,34 @@ class PagedKVCacheB200:
         for p in s.pages[keep:]:
             self._drop(p)
         del s.pages[keep:]
+        s.gone = {w: min(end, keep) for w, end in s.gone.items() if min(end, keep) > self._sink_pages(*w[1:])}
         s.length = length
         s.changed()
 
     def evict(self, seq: int, window: int, sinks: int = 0, frame_tokens: int = 1) -> int:
         """Give up the pages that no later token of the session can see under this window: all
         their tokens are before the window of the next token's frame and behind the sink frames.
-        Returns how many."""
+        Returns how many.  Tokens of an earlier frame, written anew, would see them: such a step is
+        refused (so evict after the newest frame's last rewrite).  Attention under a wider window does
+        not see what has gone."""
         s = self._get(seq)
         if window < 1 or sinks < 0 or frame_tokens < 1:
             raise ValueError("window and frame_tokens must be >= 1, sinks >= 0")
         start = max(0, s.length // frame_tokens - window + 1) * frame_tokens
-        first = -(-sinks * frame_tokens // self.page_tokens)
-        gone = [i for i in range(first, start // self.page_tokens) if s.pages[i] >= 0]
+        end = start // self.page_tokens
+        gone = [i for i in range(self._sink_pages(sinks, frame_tokens), end) if s.pages[i] >= 0]
         for i in gone:
             self._drop(s.pages[i])
             s.pages[i] = -1
         if gone:
+            w = (window, sinks, frame_tokens)
+            s.gone[w] = max(end, s.gone.get(w, 0))
             s.changed()
         return len(gone)
+
+    def _sink_pages(self, sinks: int, frame_tokens: int) -> int:
+        """Pages that the sink frames reach into."""
+        return -(-sinks * frame_tokens // self.page_tokens)
 
     # -- device work ---------------------------------------------------------------------
     def copy_pages(self, src, dst, stream=None) -> None:
@@ -612,6 +624,10 @@ class PagedKVCacheB200:
         for s, first, length in wants:
             shared = []
             if first < length:
+                for (window, _, frame), end in s.gone.items():
+                    if (first // frame - window + 1) * frame < end * pt:
+                        raise ValueError(f"token {first} sees an evicted page: its session was evicted under a window "
+                                         f"of {window} frames of {frame} for later frames")
                 for i in range(first // pt, min(-(-length // pt), len(s.pages))):
                     p = s.pages[i]
                     if p < 0:
@@ -734,7 +750,7 @@ class PagedKVCacheB200:
         if held:
             copy_pages(other.k, other.v, held, dst, to=(self.k, self.v), stream=stream)
         taken = iter([self._take() for _ in held])
-        return self._put(_Stream([next(taken) if p >= 0 else -1 for p in s.pages], s.length))
+        return self._put(_Stream([next(taken) if p >= 0 else -1 for p in s.pages], s.length, s.gone))
 
     # -- a layer's operators on a step -----------------------------------------------------
     def _live(self, batch: PagedBatchB200) -> None:

@@ -668,3 +668,36 @@ def test_session_end_to_end(pkg, cuda):
     cache, kept = other, cache
     advance([moved])
     assert kept.free_pages > 0
+
+
+def test_attention_after_evictions_sees_the_whole_window(pkg, cuda):
+    """Evict before each frame, write the frame several times (solver steps): attention agrees with the whole
+    history; rewrites that reach behind the eviction are refused."""
+    h, d, frame, window, sinks = 2, 64, 20, 3, 1
+    f = pkg.rope_axis_freqs((64,), device=cuda)
+    g = torch.Generator(device=cuda).manual_seed(5)
+    cache = pkg.PagedKVCacheB200(1, 40, kv_heads=h, head_dim=d, device=cuda)
+    a = cache.new()
+    keys, values = [], []
+    for i in range(9):
+        cache.evict(a, window, sinks, frame)
+        pos = torch.arange(i * frame, (i + 1) * frame, device=cuda, dtype=torch.int32)[:, None]
+        for rewrite in (False, True, True):
+            q, k, v = torch.randn(3, frame, h, d, device=cuda, generator=g).bfloat16()
+            plan = cache.step([a], frame, extend=not rewrite)
+            qo = cache.append(0, plan, q, k, v, pos, f, axes=(64,), norm=False)
+            out = cache.attend(0, plan, qo, window=window, sinks=sinks, frame_tokens=frame)
+            q2, k2 = pkg.qk_norm_rope(q, k, pos, f, axes=(64,), norm=False)
+            keys[i:], values[i:] = [k2], [v]
+            n = (i + 1) * frame
+            kp, vp = (torch.nn.functional.pad(torch.cat(z), (0, 0, 0, 0, 0, -n % 16)).unflatten(0, (-1, 16)).transpose(1, 2)
+                      for z in (keys, values))
+            ref = attn_ref(q2, kp, vp, torch.arange(kp.shape[0], device=cuda)[None].int(), [n], [0, frame], window,
+                           sinks, frame, d ** -0.5)
+            check(out, ref[0], attn_tol(ref, BF, d))
+    assert cache.pages_of(a).count(-1) > 3
+    with pytest.raises(ValueError, match="evicted page"):
+        cache.step([a], 2 * frame, extend=False)
+    cache.truncate(a, 8 * frame - 5)
+    with pytest.raises(ValueError, match="evicted page"):
+        cache.step([a], 5)

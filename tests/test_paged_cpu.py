@@ -164,6 +164,99 @@ def test_plans_of_forked_sessions_and_of_other_caches(pkg):
             call()
 
 
+def seen_pages(plan, row, first, window, sinks, frame):
+    """The plan's page entries that hold tokens visible to the query at position `first`."""
+    n = int(plan.kv_len[row])
+    end = min((first // frame + 1) * frame, n)
+    start = max(0, (first // frame - window + 1) * frame)
+    tokens = [j for j in range(end) if j >= start or j < sinks * frame]
+    return [int(plan.page_table[row, i]) for i in sorted({j // 16 for j in tokens})]
+
+
+@pytest.mark.parametrize("window,sinks,frame,length", [(2, 1, 20, 120), (3, 0, 16, 96), (2, 0, 10, 95), (40, 5, 1, 100)])
+def test_evicted_pages_are_not_in_sight_of_any_step(pkg, window, sinks, frame, length):
+    """After an eviction every step that is taken sees all it should; one that would not is refused."""
+    c = make(pkg, pages=20)
+    a = c.new()
+    c.step([a], length)
+    assert c.evict(a, window, sinks, frame) > 0
+    b = c.fork(a)[0]
+    before = (c.pages_of(a), list(c._refs), list(c._free), c.length(a))
+    refused = 0
+    for n in range(1, 2 * frame + 18):  # the last n tokens again
+        try:
+            plan = c.step([a], n, extend=False)
+        except ValueError as e:
+            assert "evicted page" in str(e)
+            refused += 1
+            continue
+        for first in range(length - n, length):
+            assert min(seen_pages(plan, 0, first, window, sinks, frame)) >= 0
+    assert refused
+    # what the eviction was for goes on: later tokens, and those again; the fork remembers as well
+    for s in (a, b):
+        done = c.step([s], 7)
+        again = c.step([s], 7, extend=False)
+        for plan in (done, again):
+            for first in range(length, length + 7):
+                assert min(seen_pages(plan, 0, first, window, sinks, frame)) >= 0
+    with pytest.raises(ValueError, match="evicted page"):
+        c.step([b], 2 * frame + 24, extend=False)
+    assert before[3] == length and c.length(a) == c.length(b) == length + 7
+    owned(c)
+
+
+def test_refused_step_after_eviction_changes_nothing(pkg):
+    c = make(pkg, pages=20)
+    a, b = c.new(), c.new()
+    c.step([a, b], [120, 10])
+    assert c.evict(a, window=2, sinks=1, frame_tokens=20) == 4  # pages 2..5: frame 6 sees 100 and later
+    plan = c.step([b], 1)
+    before = (c.pages_of(a), c.pages_of(b), list(c._refs), list(c._free), c.length(a), c.length(b))
+    for seqs, tokens in (([b, a], [5, 20]), ([a], [20])):  # frame 5 sees frame 4 (80 .. 99)
+        with pytest.raises(ValueError, match="evicted page"):
+            c.step(seqs, tokens, extend=False)
+    assert before == (c.pages_of(a), c.pages_of(b), list(c._refs), list(c._free), c.length(a), c.length(b))
+    assert not plan.stale
+    owned(c)
+
+
+def test_evict_truncate_step(pkg):
+    """Rejected frames are generated anew: refused where they see what was evicted, and not otherwise."""
+    c = make(pkg, pages=20)
+    a = c.new()
+    c.step([a], 120)
+    c.evict(a, window=2, frame_tokens=20)  # the next frame is 6: pages 0..5 (tokens 0..95) go
+    assert c.pages_of(a) == [-1] * 6 + c.pages_of(a)[6:]
+    c.truncate(a, 100)
+    with pytest.raises(ValueError, match="evicted page"):
+        c.step([a], 20)  # frame 5 sees frame 4
+    assert c.length(a) == 100
+    c.truncate(a, 0)  # all of it goes, and with it what was evicted
+    plan = c.step([a], 40)
+    assert min(plan.page_table[0].tolist()) >= 0
+    owned(c)
+
+
+def test_evictions_under_different_windows(pkg):
+    """A session is held to the windows under which its pages went, not to others."""
+    c = make(pkg, pages=20)
+    a = c.new()
+    c.step([a], 100)
+    assert c.evict(a, window=31, sinks=20) == 2      # pages 2, 3; the sinks' 0, 1 stay
+    assert c.evict(a, window=31) == 2                # no sinks any more
+    assert c.pages_of(a)[:5] == [-1] * 4 + c.pages_of(a)[4:5]
+    c.step([a], 6, extend=False)                     # token 94 sees from 64 on
+    with pytest.raises(ValueError, match="evicted page"):
+        c.step([a], 7, extend=False)                 # token 93 sees token 63
+    c.step([a], 1)
+    assert c.evict(a, window=5) == 2                 # the next token (101) sees from 97 on
+    c.step([a], 1, extend=False)
+    with pytest.raises(ValueError, match="evicted page"):
+        c.step([a], 6, extend=False)                 # token 95 sees from 91 on
+    owned(c)
+
+
 @pytest.mark.parametrize("bad", ["twice", "none", "unknown", "negative", "few", "rewrite"])
 def test_step_refusals(pkg, bad):
     c = make(pkg)
