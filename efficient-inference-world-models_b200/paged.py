@@ -614,13 +614,14 @@ class PagedKVCacheB200:
         """Raw page copies (the book is not touched): see :func:`copy_pages`."""
         copy_pages(self.k, self.v, src, dst, stream=stream)
 
-    def _own(self, wants: Sequence[Tuple[_Stream, int, int]], stream) -> None:
-        """For every (session, first, length): make the pages of tokens first..length-1 exist and
-        belong to the session alone, copying shared ones that hold tokens to keep."""
+    def _own(self, wants: Sequence[Tuple[_Stream, int, int]]) -> Tuple[List[List[int]], List[int], List[int], int]:
+        """For every (session, first, length): its pages when those of tokens first..length-1 exist and
+        belong to the session alone, shared ones that hold tokens to keep copied.  Returns the page lists, the
+        copies (sources, destinations) and how many free pages that takes; changes nothing."""
         pt = self.page_tokens
         refs = dict()  # what the references will be: a shared page's last sharer writes in place
-        need = 0
-        plan: List[Tuple[_Stream, List[int], int]] = []
+        src, dst, taken = [], [], 0
+        lists: List[List[int]] = []
         for s, first, length in wants:
             shared = []
             if first < length:
@@ -635,23 +636,20 @@ class PagedKVCacheB200:
                     if refs.setdefault(p, self._refs[p]) > 1:
                         refs[p] -= 1
                         shared.append(i)
-            fresh = max(0, -(-length // pt) - len(s.pages))
-            need += fresh + len(shared)
-            plan.append((s, shared, fresh))
-        if need > len(self._free):
-            raise RuntimeError(f"paged KV cache: {need} pages needed, {len(self._free)} free")
-        src, dst = [], []
-        for s, shared, fresh in plan:
-            for i in shared:
-                old, s.pages[i] = s.pages[i], self._take()
-                src.append(old)
-                dst.append(s.pages[i])
-                self._drop(old)
-            s.pages.extend(self._take() for _ in range(fresh))
-            if shared or fresh:
-                s.changed()
-        if src:
-            self.copy_pages(src, dst, stream)
+            pages = list(s.pages)
+            new = len(shared) + max(0, -(-length // pt) - len(pages))
+            free = self._free[max(0, len(self._free) - taken - new): len(self._free) - taken][::-1]  # as _take will
+            taken += new
+            if taken <= len(self._free):
+                for i, p in zip(shared, free):
+                    src.append(pages[i])
+                    dst.append(p)
+                    pages[i] = p
+                pages.extend(free[len(shared):])
+            lists.append(pages)
+        if taken > len(self._free):
+            raise RuntimeError(f"paged KV cache: {taken} pages needed, {len(self._free)} free")
+        return lists, src, dst, taken
 
     def step(self, seqs: Sequence[int], tokens: Union[int, Sequence[int]], *, extend: bool = True,
              table_width: Optional[int] = None, into: Optional[PagedBatchB200] = None,
@@ -683,11 +681,8 @@ class PagedKVCacheB200:
             raise ValueError(f"the plan is for {into.sequences} sessions and {into.tokens} tokens")
         if width * pt > 0x3fffffff:
             raise ValueError("more than 2^30 - 1 tokens in a session")
-        self._own([(s, m - n, m) for s, n, m in zip(streams, counts, lengths)], stream)
-        for s, m in zip(streams, lengths):
-            if m != s.length:
-                s.length = m
-                s.changed()
+        # everything that can fail comes before the book changes
+        lists, src, dst, taken = self._own([(s, m - n, m) for s, n, m in zip(streams, counts, lengths)])
         n = len(seqs)
         host = np.full(2 * n + 1 + n * width + total, -1, np.int32)
         cu = host[: n + 1]
@@ -696,17 +691,27 @@ class PagedKVCacheB200:
         host[n + 1: 2 * n + 1] = lengths
         table = host[2 * n + 1: 2 * n + 1 + n * width].reshape(n, width)
         slots = host[2 * n + 1 + n * width:]
-        for i, (s, c, m) in enumerate(zip(streams, counts, lengths)):
-            table[i, : len(s.pages)] = s.pages
+        for i, (pages, c, m) in enumerate(zip(lists, counts, lengths)):
+            table[i, : len(pages)] = pages
             at = np.arange(m - c, m)
             slots[cu[i]: cu[i + 1]] = table[i, at // pt].astype(np.int64) * pt + at % pt
         b = into if into is not None else PagedBatchB200(n, total, width, pt, self.device)
+        if src:
+            self.copy_pages(src, dst, stream)
         there = _elsewhere(self.device, stream)
         if there is not None:
             with there:
                 b._buffer.copy_(torch.from_numpy(host))
         else:
             b._buffer.copy_(torch.from_numpy(host))
+        for _ in range(taken):
+            self._take()
+        for p in src:
+            self._drop(p)
+        for s, pages, m in zip(streams, lists, lengths):
+            if m != s.length or pages != s.pages:
+                s.pages, s.length = pages, m
+                s.changed()
         b.max_q = max(max(counts), b.max_q)  # a captured launch keeps the bound it was captured with
         b.cache = weakref.ref(self)
         for i in b.seqs:  # a rebuilt plan no longer follows its earlier sessions

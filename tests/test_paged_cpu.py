@@ -257,6 +257,47 @@ def test_evictions_under_different_windows(pkg):
     owned(c)
 
 
+@pytest.mark.parametrize("where", ["copy", "plan", "upload", "rebuild"])
+def test_step_that_raises_changes_nothing(pkg, monkeypatch, where):
+    """A failing copy, plan allocation or upload leaves the book and the plans as they were."""
+    c = make(pkg, pages=20)
+    a = c.new()
+    c.step([a], 40)
+    fill(c, a, 0, range(40))
+    b, d = c.fork(a, 2)
+    live = c.step([d], 0)
+    old = c.step([a, b], [0, 0], table_width=5)
+
+    def book():
+        return ([(c.pages_of(x), c.length(x)) for x in (a, b, d)], list(c._refs), list(c._free), live.stale,
+                old.stale, old.seqs, old.kv_len.tolist(), old.page_table.tolist(), read(c, a), read(c, b), read(c, d))
+
+    before = book()
+
+    def fail(*args, **kw):
+        raise RuntimeError("planted")
+
+    copy = c.copy_pages
+    with monkeypatch.context() as m:
+        if where == "copy":
+            m.setattr(c, "copy_pages", fail)
+        elif where == "plan":
+            m.setattr(pkg.paged, "PagedBatchB200", fail)
+        else:
+            m.setattr(torch, "from_numpy", fail)
+        with pytest.raises(RuntimeError, match="planted"):
+            if where == "rebuild":
+                c.step([a, b], [0, 0], into=old, extend=True)
+            else:
+                c.step([a, b, d], [3, 20, 0])
+    assert before == book()
+    owned(c)
+    assert c.copy_pages is copy
+    c.step([a, b, d], [3, 20, 0])  # and it goes on from there
+    assert read(c, a)[:40] == read(c, b)[:40] == read(c, d) == [float(i) for i in range(40)]
+    owned(c)
+
+
 @pytest.mark.parametrize("bad", ["twice", "none", "unknown", "negative", "few", "rewrite"])
 def test_step_refusals(pkg, bad):
     c = make(pkg)
