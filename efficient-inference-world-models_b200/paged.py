@@ -22,6 +22,7 @@ The reference keeps whole tensors per session and concatenates each new frame
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import struct
 import weakref
@@ -658,8 +659,9 @@ class PagedKVCacheB200:
         With ``extend=False`` the step's tokens are the sessions' last ones again (the same frame
         at another solver step: its keys and values are written anew).  Pages are taken, and
         shared ones that the step writes into are copied first.  ``table_width``: pages per session
-        the plan has room for (default: what this step needs).  ``into``: rebuild this plan in place, on the current
-        stream, for the same number of sessions and tokens."""
+        the plan has room for (default: what this step needs).  ``into``: rebuild this plan in place, on ``stream``
+        (default: the current one), for the same number of sessions and tokens.  A new plan's memory belongs to
+        that stream."""
         seqs = [int(i) for i in seqs]
         if not seqs or len(set(seqs)) != len(seqs):
             raise ValueError("a step takes one or more different sessions")
@@ -695,14 +697,10 @@ class PagedKVCacheB200:
             table[i, : len(pages)] = pages
             at = np.arange(m - c, m)
             slots[cu[i]: cu[i + 1]] = table[i, at // pt].astype(np.int64) * pt + at % pt
-        b = into if into is not None else PagedBatchB200(n, total, width, pt, self.device)
-        if src:
-            self.copy_pages(src, dst, stream)
-        there = _elsewhere(self.device, stream)
-        if there is not None:
-            with there:
-                b._buffer.copy_(torch.from_numpy(host))
-        else:
+        with _elsewhere(self.device, stream) or contextlib.nullcontext():  # a new plan's memory is the stream's, too
+            b = into if into is not None else PagedBatchB200(n, total, width, pt, self.device)
+            if src:
+                self.copy_pages(src, dst)
             b._buffer.copy_(torch.from_numpy(host))
         for _ in range(taken):
             self._take()

@@ -701,3 +701,33 @@ def test_attention_after_evictions_sees_the_whole_window(pkg, cuda):
     cache.truncate(a, 8 * frame - 5)
     with pytest.raises(ValueError, match="evicted page"):
         cache.step([a], 5)
+
+
+def test_step_on_another_stream(pkg, cuda):
+    """step(stream=) makes the plan on that stream: work queued on the current stream keeps its memory."""
+    cache = pkg.PagedKVCacheB200(1, 512, kv_heads=1, head_dim=64, device=cuda)
+    side = torch.cuda.Stream(device=cuda)
+    seqs = [cache.new() for _ in range(64)]
+    n = 2 * 64 + 1 + 64 * 40 + 64  # the size of the plan's buffer
+    kept = torch.empty(n, dtype=torch.int32, device=cuda)
+    for _ in range(4):
+        block = torch.arange(n, dtype=torch.int32, device=cuda)
+        torch.cuda._sleep(50_000_000)
+        kept.copy_(block)  # queued: reads the block after it was given back
+        at = block.data_ptr()
+        del block
+        plan = cache.step(seqs, 1, table_width=40, stream=side)
+        assert plan._buffer.data_ptr() != at
+        torch.cuda.synchronize()
+        assert torch.equal(kept, torch.arange(n, dtype=torch.int32, device=cuda))
+        assert plan.kv_len.tolist() == [cache.length(s) for s in seqs]
+        assert plan.page_table[:, 0].tolist() == [cache.pages_of(s)[0] for s in seqs]
+    # append and attend follow on the same stream
+    f = pkg.rope_axis_freqs((64,), device=cuda)
+    q, k, v = torch.randn(3, 64, 1, 64, device=cuda).bfloat16()
+    pos = torch.zeros(64, 1, dtype=torch.int32, device=cuda)
+    side.wait_stream(torch.cuda.current_stream())
+    qo = cache.append(0, plan, q, k, v, pos, f, axes=(64,), norm=False, stream=side)
+    out = cache.attend(0, plan, qo, window=1, stream=side)
+    side.synchronize()
+    assert torch.equal(out, v)  # a token that sees itself alone

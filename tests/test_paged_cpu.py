@@ -298,6 +298,32 @@ def test_step_that_raises_changes_nothing(pkg, monkeypatch, where):
     owned(c)
 
 
+def test_plan_is_allocated_under_the_given_stream(pkg, monkeypatch):
+    """The plan's memory belongs to the stream that fills it."""
+    c = make(pkg)
+    a = c.new()
+    inside, made = [], []
+
+    class Context:
+        def __enter__(self):
+            inside.append(True)
+
+        def __exit__(self, *exc):
+            inside.pop()
+
+    plan = pkg.paged.PagedBatchB200
+
+    def make_plan(*args):
+        made.append(bool(inside))
+        return plan(*args)
+
+    monkeypatch.setattr(pkg.paged, "_elsewhere", lambda device, stream: Context() if stream else None)
+    monkeypatch.setattr(pkg.paged, "PagedBatchB200", make_plan)
+    c.step([a], 3, stream="another")
+    c.step([a], 3)
+    assert made == [True, False]
+
+
 @pytest.mark.parametrize("bad", ["twice", "none", "unknown", "negative", "few", "rewrite"])
 def test_step_refusals(pkg, bad):
     c = make(pkg)
