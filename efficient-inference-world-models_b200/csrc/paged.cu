@@ -29,6 +29,8 @@ int pages_check(const oasis_pages_t* p, const char* who) {
 // piece of successive pairs are neighbours, so a source copied to several forks comes from
 // L2 after its first read.  Bound by HBM, every byte read once and written once: 1,500 pages of 16
 // layers (3.1 GB) take 467 us, 6.7 TB/s; one page of 16 layers (2 MB) 2.4 us.
+// The pointers are not __restrict__: that would let the sources be read through the read-only path, and
+// with dependent launches the kernel that appends to the pages may still run when this one starts.
 // ----------------------------------------------------------------------------------
 constexpr int kCopyThreads = 256;
 constexpr int kCopyVecs = 8;                                     // 16-byte vectors per thread
@@ -41,9 +43,8 @@ struct PagePairs {
 
 template <int N>
 __global__ void __launch_bounds__(kCopyThreads)
-    pages_copy_kernel(const __grid_constant__ PagePairs<N> pairs, int n, const uint8_t* __restrict__ sk,
-                      const uint8_t* __restrict__ sv, uint8_t* __restrict__ dk, uint8_t* __restrict__ dv,
-                      int src_pages, int dst_pages, long long page_bytes, int pieces) {
+    pages_copy_kernel(const __grid_constant__ PagePairs<N> pairs, int n, const uint8_t* sk, const uint8_t* sv,
+                      uint8_t* dk, uint8_t* dv, int src_pages, int dst_pages, long long page_bytes, int pieces) {
   pdl_trigger();
   pdl_wait();
   // blockIdx.x = ((layer * 2 + tensor) * pieces + piece) * n + pair

@@ -731,3 +731,31 @@ def test_step_on_another_stream(pkg, cuda):
     out = cache.attend(0, plan, qo, window=1, stream=side)
     side.synchronize()
     assert torch.equal(out, v)  # a token that sees itself alone
+
+
+def test_copies_follow_appends_back_to_back(pkg, cuda):
+    """A page copy, an append into the copy, a copy of that: each sees what the launch before it stored."""
+    hk, d, pt, n = 8, 128, 16, 64
+    f = pkg.rope_axis_freqs((d,), device=cuda)
+    pos = torch.zeros(n * pt, 1, dtype=torch.int32, device=cuda)
+    kp, vp = (torch.zeros(4 * n, hk, pt, d, dtype=BF, device=cuda) for _ in range(2))
+    first, second, third = (list(range(i * n, (i + 1) * n)) for i in range(3))
+    at = torch.arange(n * pt, dtype=torch.int32, device=cuda)
+    slots = [at + i * n * pt for i in range(3)]
+    x = [torch.randn(3, n * pt, hk, d, device=cuda).bfloat16() for _ in range(6)]
+    got = []
+    for i in range(0, 6, 2):
+        for (q, k, v), to in ((x[i], 0), (x[i + 1], 1)):
+            pkg.qk_norm_rope_append(q, k, v, pos, f, kp, vp, slots[to], axes=(d,), norm=False)
+            pkg.copy_pages(kp, vp, first if to == 0 else second, second if to == 0 else third)
+        got.append((kp.clone(), vp.clone()))
+
+    def as_pages(z):  # position 0 turns nothing
+        return z.unflatten(0, (n, pt)).transpose(1, 2)
+
+    for i, (k, v) in zip(range(0, 6, 2), got):
+        for pages, which in ((k, 1), (v, 2)):
+            assert torch.equal(pages[:n], as_pages(x[i][which]))
+            assert torch.equal(pages[n: 2 * n], as_pages(x[i + 1][which]))
+            assert torch.equal(pages[2 * n: 3 * n], as_pages(x[i + 1][which]))
+            assert not pages[3 * n:].any()
