@@ -14,7 +14,7 @@ Functions over plain tensors (each one call into ``liboasis_b200.so`` on the cur
 pages until one of them writes (copy on write), eviction frees what the window has left behind,
 compaction moves the used pages to the front.  :class:`PagedBatchB200` is one step's plan.
 
-The operators compute results only (no gradients): inputs that require gradients are refused.
+The operators compute results only: tensors that require gradients, or carry forward-mode tangents, are refused.
 The reference keeps whole tensors per session and concatenates each new frame
 (``kv_cache/manager.py:246-306``, ``:416-480``) and branches by copying all of it
 (``snapshot``/``restore``, ``:555-588``).
@@ -30,6 +30,7 @@ from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 from .kv_cache import HEAD_DIM, HEADS
@@ -54,6 +55,11 @@ def _entry(name: str):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _dual_level() -> bool:
+    """Whether tensors may carry forward-mode tangents."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
 
 
 # Every function first looks at its arguments with one cheap condition; where that does not
@@ -87,10 +93,10 @@ def _heads3(name: str, t: torch.Tensor) -> None:
 
 
 def _no_grad(*tensors) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError("no gradient is computed here: detach the inputs or use torch.no_grad()")
+    grad, dual = torch.is_grad_enabled(), _dual_level()
+    for t in tensors:
+        if t is not None and (grad and t.requires_grad or dual and forward_ad.unpack_dual(t).tangent is not None):
+            raise ValueError("no gradient is computed here: detach the inputs or use torch.no_grad()")
 
 
 def _index32(name: str, t: torch.Tensor, shape, device) -> None:
@@ -161,12 +167,13 @@ def _rope_checks(q, k, v, positions, freqs, q_weight, k_weight, axes, norm, k_pa
         if k_pages.shape[1] != k.shape[1] or k_pages.shape[3] != d or k_pages.dtype != k.dtype:
             raise ValueError("the pages do not fit the keys (kv_heads, head_dim, type)")
         _index32("slots", slots, (tokens,), dev)
-    _no_grad(q, k, v, q_weight, k_weight, k_pages, v_pages)
+    _no_grad(q, k, v, freqs, q_weight, k_weight, k_pages, v_pages)
 
 
 def _out_check(name: str, out: torch.Tensor, like: torch.Tensor) -> None:
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{name} must have its input's shape, type and device")
+    _no_grad(out)
     _heads3(name, out)
     if any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
         raise ValueError(f"{name} must not be an expanded tensor: its rows are one memory")
@@ -184,7 +191,8 @@ def _rope(q, k, v, positions, freqs, k_pages, v_pages, slots, axes, interleaved,
             and 1 <= n_axes <= 4 and (pt is torch.int32 or pt is torch.int64) and ph == (qh[0], n_axes)
             and freqs.dtype is torch.float64 and freqs.dim() == 1 and 2 * freqs.numel() == sum(axes)
             and positions.is_contiguous() and freqs.is_contiguous()
-            and not (q.requires_grad or k.requires_grad) and q_weight is not None and k_weight is not None and norm
+            and not (q.requires_grad or k.requires_grad or freqs.requires_grad or _dual_level())
+            and q_weight is not None and k_weight is not None and norm
             and q_weight.dtype is k_weight.dtype is torch.float32 and q_weight.shape == k_weight.shape == qh[2:]
             and q_weight.get_device() == k_weight.get_device() == dev
             and q_weight.is_contiguous() and k_weight.is_contiguous()
@@ -346,7 +354,7 @@ def attn_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, p
             and (qh[0] == th[0] if cu_q is None else cu_q.get_device() == dev and cu_q.dtype is torch.int32
                  and cu_q.shape == (th[0] + 1,) and cu_q.is_contiguous())
             and (window is None or window >= 1) and sinks >= 0 and frame_tokens >= 1
-            and not (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad)):
+            and not (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or _dual_level())):
         _attn_checks(q, k_pages, v_pages, page_table, kv_len, cu_q, window, sinks, frame_tokens)
     tokens, heads, d = qh
     qs0, qs1, _ = q.stride()
@@ -411,7 +419,7 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src, dst, *, to=Non
     if not (dev >= 0 and dev == v_pages.get_device() and kh == v_pages.shape and dt == v_pages.dtype
             and 4 <= len(kh) <= 5 and (dt is torch.bfloat16 or dt is torch.float16)
             and k_pages.is_contiguous() and v_pages.is_contiguous()
-            and not (k_pages.requires_grad or v_pages.requires_grad)):
+            and not (k_pages.requires_grad or v_pages.requires_grad or _dual_level())):
         _cuda("k_pages", k_pages)
         _cuda("v_pages", v_pages, k_pages.device)
         _pages(k_pages, v_pages, (4, 5))

@@ -759,3 +759,39 @@ def test_copies_follow_appends_back_to_back(pkg, cuda):
             assert torch.equal(pages[n: 2 * n], as_pages(x[i + 1][which]))
             assert torch.equal(pages[2 * n: 3 * n], as_pages(x[i + 1][which]))
             assert not pages[3 * n:].any()
+
+
+def test_gradients_are_refused_in_every_argument(pkg, cuda):
+    """Backward and forward gradients of any input, and outputs that require them."""
+    ad = torch.autograd.forward_ad
+    q, kp, vp, table, lens, cu = attn_inputs(cuda, [4], [40], 4, 2, 64, BF, 16)
+    x, k, v, pos, wq, wk, f = rope_inputs(pkg, cuda, 4, 4, 2, 64, BF, (16, 24, 24))
+    slots = torch.arange(4, device=cuda, dtype=torch.int32)
+    kw = dict(axes=(16, 24, 24))
+
+    def attn(q=q, kp=kp, vp=vp, **kw):
+        return pkg.attn_window(q, kp, vp, table, lens, cu, **kw)
+
+    def rope(q=x, k=k, f=f, wq=wq, wk=wk, **more):
+        return pkg.qk_norm_rope(q, k, pos, f, q_weight=wq, k_weight=wk, **kw, **more)
+
+    def append(q=x, k=k, v=v, f=f, wq=wq, wk=wk, kp=kp, vp=vp, **more):
+        return pkg.qk_norm_rope_append(q, k, v, pos, f, kp, vp, slots, q_weight=wq, k_weight=wk, **kw, **more)
+
+    calls = [(attn, dict(q=q, kp=kp, vp=vp, out=torch.empty_like(q))),
+             (rope, dict(q=x, k=k, f=f, wq=wq, wk=wk, q_out=torch.empty_like(x), k_out=torch.empty_like(k))),
+             (append, dict(q=x, k=k, v=v, f=f, wq=wq, wk=wk, kp=kp, vp=vp, q_out=torch.empty_like(x)))]
+    for call, args in calls:
+        call()
+        for name, t in args.items():
+            leaf = t.detach().clone().requires_grad_()
+            with pytest.raises(ValueError, match="gradient"):
+                call(**{name: leaf})
+            with torch.no_grad():
+                call(**{name: leaf})
+            with ad.dual_level(), torch.no_grad():
+                call(**{name: t})
+                with pytest.raises(ValueError, match="gradient"):
+                    call(**{name: ad.make_dual(t.detach().clone(), torch.ones_like(t))})
+    with ad.dual_level(), pytest.raises(ValueError, match="gradient"):
+        pkg.copy_pages(ad.make_dual(kp, torch.ones_like(kp)), vp, [0], [1])

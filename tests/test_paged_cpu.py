@@ -362,6 +362,30 @@ def test_axis_frequencies(pkg):
             pkg.rope_axis_freqs(axes, theta, device="cpu")
 
 
+def test_no_gradient_is_dropped_silently(pkg):
+    """Inputs that require gradients, backward or forward, are refused."""
+    check = pkg.paged._no_grad
+    x = torch.zeros(4, 2, 64)
+    check(x, None)
+    with pytest.raises(ValueError, match="gradient"):
+        check(x, x.clone().requires_grad_())
+    with torch.no_grad():
+        check(x.clone().requires_grad_())
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        check(x, None)
+        with pytest.raises(ValueError, match="gradient"):
+            check(x, dual)
+        with torch.no_grad(), pytest.raises(ValueError, match="gradient"):
+            check(dual)  # tangents pass through no_grad
+        check(torch.autograd.forward_ad.unpack_dual(dual).primal)
+    out = x.clone().requires_grad_()
+    with pytest.raises(ValueError, match="gradient"):
+        pkg.paged._out_check("out", out, x)
+    with torch.no_grad():
+        pkg.paged._out_check("out", out, x)
+
+
 # ---------------------------------------------------------------- refusals of the C entry points
 
 
