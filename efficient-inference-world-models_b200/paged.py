@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import operator
 import struct
 import weakref
 from typing import Dict, List, Optional, Sequence, Tuple, Union
@@ -562,6 +563,7 @@ class PagedKVCacheB200:
         into a shared page first gets a copy of it.  No device work.  Plans that write into ``seq`` are
         out of date from here on: their slots are shared now."""
         s = self._get(seq)
+        copies = operator.index(copies)
         if copies < 0:
             raise ValueError("copies must be >= 0")
         if copies:

@@ -324,6 +324,19 @@ def test_plan_is_allocated_under_the_given_stream(pkg, monkeypatch):
     assert made == [True, False]
 
 
+def test_fork_takes_whole_numbers(pkg):
+    c = make(pkg)
+    a = c.new()
+    c.step([a], 20)
+    before = (c.sessions, list(c._refs), list(c._free))
+    for copies in (1.5, "2", None, -1):
+        with pytest.raises((TypeError, ValueError)):
+            c.fork(a, copies)
+    assert before == (c.sessions, list(c._refs), list(c._free))
+    assert len(c.fork(a, np.int64(2))) == 2
+    owned(c)
+
+
 @pytest.mark.parametrize("bad", ["twice", "none", "unknown", "negative", "few", "rewrite"])
 def test_step_refusals(pkg, bad):
     c = make(pkg)
