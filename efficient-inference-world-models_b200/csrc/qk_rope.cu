@@ -309,6 +309,10 @@ extern "C" int oasis_qk_norm_rope(const oasis_qk_norm_rope_t* p, cudaStream_t st
     if (p->pages->layers != 1 || p->pages->kv_heads != p->kv_heads || p->pages->head_dim != d ||
         p->pages->dtype != p->dtype)
       return fail(OASIS_ERR_INVALID_ARG, std::string(who) + ": the pages do not fit the keys (one layer, heads, head_dim, type)");
+    const uintptr_t kb = reinterpret_cast<uintptr_t>(p->pages->k), vb = reinterpret_cast<uintptr_t>(p->pages->v);
+    const uintptr_t pool = static_cast<uintptr_t>(p->pages->pages) * p->pages->kv_heads * p->pages->page_tokens * d * 2;
+    if (kb < vb + pool && vb < kb + pool)
+      return fail(OASIS_ERR_INVALID_ARG, std::string(who) + ": key and value pages overlap");
   } else if (!p->k_out) {
     return fail(OASIS_ERR_INVALID_ARG, std::string(who) + ": null pointer");
   }

@@ -171,15 +171,84 @@ def _rope_checks(q, k, v, positions, freqs, q_weight, k_weight, axes, norm, k_pa
     _no_grad(q, k, v, freqs, q_weight, k_weight, k_pages, v_pages)
 
 
-def _out_check(name: str, out: torch.Tensor, like: torch.Tensor) -> None:
-    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
-        raise ValueError(f"{name} must have its input's shape, type and device")
-    _no_grad(out)
-    _heads3(name, out)
-    if any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
+def _starts(t: torch.Tensor) -> np.ndarray:
+    """Byte addresses of a view's [tokens][heads] runs of head_dim elements."""
+    (n, h, _), (ts, hs, _), e = t.shape, t.stride(), t.element_size()
+    return t.data_ptr() + e * (ts * np.arange(n)[:, None] + hs * np.arange(h)).ravel()
+
+
+def _extent(shape, strides, size: int) -> int:
+    """Bytes from a tensor's first element to behind its last."""
+    n = 1
+    for m, st in zip(shape, strides):
+        if m == 0:
+            return 0
+        n += st * (m - 1)
+    return n * size
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [tokens][heads][head_dim] views (head_dim contiguous), or such a view and a contiguous tensor, have
+    memory in common.  Exact: columns of one projection interleave and have none."""
+    x, y, e = a.data_ptr(), b.data_ptr(), a.element_size()
+    sa, sb, ta, tb = a.shape, b.shape, a.stride(), b.stride()
+    if x >= y + _extent(sb, tb, b.element_size()) or y >= x + _extent(sa, ta, e):
+        return False
+    step = ta[0] * e
+    same_step = step > 0 and len(sb) == 3 and step == tb[0] * e
+    if same_step:  # the usual case: each token's heads lie in a part of the step of their own
+        at = (y - x) % step
+        if at >= _extent(sa[1:], ta[1:], e) and at + _extent(sb[1:], tb[1:], e) <= step:
+            return False
+    if a.is_contiguous() and b.is_contiguous():
+        return True
+    a, b = (t if t.dim() == 3 else t.view(1, 1, -1) for t in (a, b))
+    da, db = (t.shape[2] * t.element_size() for t in (a, b))
+    if same_step:
+        # runs of token i and head j of a, token k and head l of b: only i - k counts; for each of the heads the
+        # nearest multiples of the step that are within the tokens
+        gap = _starts(b[:1])[None] - _starts(a[:1])[:, None]
+        lo, hi = 1 - b.shape[0], a.shape[0] - 1
+        near = gap // step
+        return any(bool(((off > -db) & (off < da)).any())
+                   for u in (near, near + 1) for off in (gap - step * np.clip(u, lo, hi),))
+    first, second = _starts(a), np.sort(_starts(b))  # any strides
+    at = np.searchsorted(second, first)
+    before, after = second[np.maximum(at - 1, 0)], second[np.minimum(at, len(second) - 1)]
+    return bool((((before <= first) & (before + db > first)) | ((after >= first) & (after < first + da))).any())
+
+
+def _folds(t: torch.Tensor) -> bool:
+    """Whether a view's rows lie over one another."""
+    (n, h, d), (ts, hs, _) = t.shape, t.stride()
+    for (n1, s1), (n2, s2) in (((n, ts), (h, hs)), ((h, hs), (n, ts))):
+        if (n2 <= 1 or s2 >= d) and (n1 <= 1 or s1 >= (s2 * (n2 - 1) if n2 > 1 else 0) + d):
+            return False  # the usual layouts: one dimension's rows lie within a step of the other
+    at = np.sort(_starts(t))
+    return bool((np.diff(at) < d * t.element_size()).any())
+
+
+def _out_check(name: str, out: torch.Tensor, like: torch.Tensor, **others: Optional[torch.Tensor]) -> None:
+    """An output given: like its input, over it exactly or not at all, and off the other tensors."""
+    if out is not like:
+        if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+            raise ValueError(f"{name} must have its input's shape, type and device")
+        _no_grad(out)
+        _heads3(name, out)
+    shape, strides = out.shape, out.stride()
+    if 0 in strides and any(st == 0 and n > 1 for st, n in zip(strides, shape)):
         raise ValueError(f"{name} must not be an expanded tensor: its rows are one memory")
-    if out.data_ptr() == like.data_ptr() and out.stride() != like.stride():
+    at = out.data_ptr()
+    if out is not like and at == like.data_ptr() and strides != like.stride():
         raise ValueError(f"{name} over its input must have the input's strides")
+    if _folds(out):
+        raise ValueError(f"{name}'s rows overlap each other")
+    end = at + _extent(shape, strides, out.element_size())
+    if out is not like and like.data_ptr() != at:
+        others["its input, except to lie over it exactly"] = like
+    for other, t in others.items():
+        if t is not None and t.data_ptr() < end and _overlap(out, t):
+            raise ValueError(f"{name} must not overlap {other}")
 
 
 def _rope(q, k, v, positions, freqs, k_pages, v_pages, slots, axes, interleaved, norm, q_weight, k_weight, eps,
@@ -215,7 +284,7 @@ def _rope(q, k, v, positions, freqs, k_pages, v_pages, slots, axes, interleaved,
         q_out = torch.empty_like(q, memory_format=_CONTIGUOUS)
         os0, os1 = heads * d, d
     else:
-        _out_check("q_out", q_out, q)
+        _out_check("q_out", q_out, q, k=k, v=v, k_pages=k_pages, v_pages=v_pages)
         os0, os1, _ = q_out.stride()
     vs0 = vs1 = vs2 = ko0 = ko1 = v_ptr = ko_ptr = pages_ptr = slots_ptr = 0
     if v is not None:
@@ -227,7 +296,7 @@ def _rope(q, k, v, positions, freqs, k_pages, v_pages, slots, axes, interleaved,
             k_out = torch.empty_like(k, memory_format=_CONTIGUOUS)
             ko0, ko1 = kh[1] * d, d
         else:
-            _out_check("k_out", k_out, k)
+            _out_check("k_out", k_out, k, q=q, q_out=None if q_out is q else q_out)
             ko0, ko1, _ = k_out.stride()
         ko_ptr = k_out.data_ptr()
     if d > 1 and (qs2 != 1 or ks2 != 1 or (v is not None and vs2 != 1)):
@@ -260,7 +329,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freq
     may be less than head_dim: the rest is only normed), ``positions`` [tokens][len(axes)] int32 or
     int64, ``freqs`` the fp64 frequencies of the pairs (:func:`rope_axis_freqs`).  Pairs are
     neighbours (``interleaved``, as the model here rotates) or halves of the rotated dims.  q_out / k_out may
-    be q / k.  Returns (q_out, k_out)."""
+    be q / k, and otherwise overlap no tensor of the call.  Returns (q_out, k_out)."""
     if stream is not None or q.get_device() != _current_device():
         there = _elsewhere(q.device, stream)
         if there is not None:
@@ -335,7 +404,8 @@ def attn_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, p
 
     ``max_q`` / ``max_kv`` (bounds on the queries and tokens of a sequence) only choose the launch; too
     small ones cost time.
-    Rows that belong to no sequence are not written.  ``out`` may be q.  Returns out, or (out, lse)
+    Rows that belong to no sequence are not written.  ``out`` may be q, and otherwise overlaps no tensor of the
+    call.  Returns out, or (out, lse)
     with lse fp32 [tokens][heads], the natural logarithm of the softmax sum."""
     dev = q.get_device()
     if stream is not None or dev != _current_device():
@@ -363,7 +433,7 @@ def attn_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, p
         out = torch.empty_like(q, memory_format=_CONTIGUOUS)
         os0, os1 = heads * d, d
     else:
-        _out_check("out", out, q)
+        _out_check("out", out, q, k_pages=k_pages, v_pages=v_pages)
         os0, os1, _ = out.stride()
     if tokens == 1:  # a dimension of one element may have any stride
         qs0 = os0 = 0

@@ -795,3 +795,25 @@ def test_gradients_are_refused_in_every_argument(pkg, cuda):
                     call(**{name: ad.make_dual(t.detach().clone(), torch.ones_like(t))})
     with ad.dual_level(), pytest.raises(ValueError, match="gradient"):
         pkg.copy_pages(ad.make_dual(kp, torch.ones_like(kp)), vp, [0], [1])
+
+
+def test_outputs_that_overlap_other_tensors_are_refused(pkg, cuda):
+    q, kp, vp, table, lens, cu = attn_inputs(cuda, [4], [40], 4, 4, 64, BF, 16)
+    x, k, v, pos, wq, wk, f = rope_inputs(pkg, cuda, 4, 4, 4, 64, BF, (64,))
+    slots = torch.arange(4, device=cuda, dtype=torch.int32)
+    shifted = torch.zeros(7, 4, 64, dtype=BF, device=cuda)
+    one = kp.view(-1, 4, 64)
+    for call in (lambda: pkg.attn_window(shifted[:4], kp, vp, table, lens, cu, out=shifted[1:5]),
+                 lambda: pkg.attn_window(q, kp, vp, table, lens, cu, out=one[:4]),
+                 lambda: pkg.qk_norm_rope(x, k, pos, f, axes=(64,), q_out=k),
+                 lambda: pkg.qk_norm_rope(x, k, pos, f, axes=(64,), k_out=x),
+                 lambda: pkg.qk_norm_rope(x, x, pos, f, axes=(64,), q_out=x, k_out=x),
+                 lambda: pkg.qk_norm_rope(x, k, pos, f, axes=(64,), q_out=shifted[:4], k_out=shifted[1:5]),
+                 lambda: pkg.qk_norm_rope_append(x, k, v, pos, f, kp, vp, slots, axes=(64,), q_out=v),
+                 lambda: pkg.qk_norm_rope_append(x, k, v, pos, f, kp, vp, slots, axes=(64,), q_out=one[:4]),
+                 lambda: pkg.qk_norm_rope_append(x, k, v, pos, f, kp, kp, slots, axes=(64,))):
+        with pytest.raises((ValueError, pkg.OasisError), match="overlap"):
+            call()
+    want = pkg.qk_norm_rope(x, k, pos, f, axes=(64,))  # in place among the columns of one projection
+    got = pkg.qk_norm_rope(x, k, pos, f, axes=(64,), q_out=x, k_out=k)
+    assert all(torch.equal(a, b) for a, b in zip(want, got)) and got[0] is x and got[1] is k

@@ -399,6 +399,51 @@ def test_no_gradient_is_dropped_silently(pkg):
         pkg.paged._out_check("out", out, x)
 
 
+def test_overlap_of_views_matches_a_count_of_elements(pkg):
+    """Random [tokens][heads][dims] views of one buffer: _overlap against the sets of their elements."""
+    rng = np.random.RandomState(0)
+    base = torch.zeros(4096, dtype=torch.bfloat16)
+    where = torch.arange(4096)
+    found = [0, 0]
+    for i in range(600):
+        views = []
+        for _ in range(2):
+            t, h, d = rng.randint(1, 6), rng.randint(1, 5), 8 * rng.randint(1, 4)
+            strides = sorted(8 * rng.randint(0, 12, 2))
+            if rng.rand() < 0.5:
+                strides.reverse()
+            if views and rng.rand() < 0.7:  # mostly of one token stride, as the columns of a projection
+                strides = [views[0][1][0], strides[1]]
+            views.append(((t, h, d), [int(x) for x in strides] + [1], int(8 * rng.randint(0, 120))))
+        a, b = (torch.as_strided(base, *v) for v in views)
+        x, y = (set(torch.as_strided(where, *v).flatten().tolist()) for v in views)
+        found[bool(x & y)] += 1
+        assert pkg.paged._overlap(a, b) == bool(x & y), views
+        assert pkg.paged._overlap(b, a) == bool(x & y), views
+        assert pkg.paged._folds(a) == (len(x) < a.numel()), views[0]
+    assert min(found) > 100
+    assert not pkg.paged._overlap(base[:0].view(0, 2, 8), base.view(-1, 2, 8))
+
+
+def test_outputs_stay_off_other_tensors(pkg):
+    qkv = torch.zeros(6, 12 * 64, dtype=torch.bfloat16)
+    q, k, v = (z.unflatten(1, (4, 64)) for z in qkv.split(4 * 64, 1))
+    check = pkg.paged._out_check
+    check("q_out", q, q, k=k, v=v)  # its own input, between the others
+    check("q_out", torch.empty_like(q), q, k=k, v=v)
+    check("q_out", torch.zeros(4, 6, 64, dtype=torch.bfloat16).transpose(0, 1), q, k=k, v=v)
+    check("k_out", k, k, q=q, q_out=q)
+    rows = torch.zeros(9, 4, 64, dtype=torch.bfloat16)
+    for out, like, others in ((k, q, dict(k=k)),                            # another input
+                              (rows[1:7], rows[:6], {}),                    # its input, one row on
+                              (rows[:6], rows[2:8], {}),
+                              (k, k, dict(q_out=k)),                        # two outputs
+                              (rows[:6], q, dict(k_pages=rows)),
+                              (torch.as_strided(rows, (6, 4, 64), (128, 64, 1)), q, {})):  # its own rows
+        with pytest.raises(ValueError, match="overlap|one memory"):
+            check("out", out, like, **others)
+
+
 # ---------------------------------------------------------------- refusals of the C entry points
 
 
@@ -463,6 +508,14 @@ def test_qk_norm_rope_append_refusals(pkg, page, change, status):
     args.update(change)
     args["pages"] = ctypes.pointer(pages(pkg, **page))
     assert pkg.lib().oasis_qk_norm_rope(rope_args(pkg, **args), None) == status
+
+
+def test_qk_norm_rope_append_refuses_one_pool_for_both(pkg):
+    """Keys and values of a slot cannot lie in the same memory (4 pages of 2 heads x 16 x 64: 16384 bytes)."""
+    for v, status in ((16, 1), (32, 1), (16 + 16384 - 16, 1)):
+        args = dict(v=16, k_out=None, slots=16, pages=ctypes.pointer(pages(pkg, v=v)))
+        assert pkg.lib().oasis_qk_norm_rope(rope_args(pkg, **args), None) == status
+        assert b"overlap" in pkg.lib().oasis_last_error()
 
 
 def test_no_tokens_launch_nothing(pkg):
