@@ -22,6 +22,7 @@ constexpr int kWtKeys = 128;     // keys of a K/V tile
 constexpr int kWtThreads = 384;  // 8 softmax warps, MMA, K loads, V loads, V looked over
 constexpr int kWtRegs = 168;     // per thread at launch (which checks it); the softmax warps take from the others
 constexpr float kWtLazy = 8.0f;  // log2 of how far scores may pass the maximum in use
+constexpr int kWtClean = 0x7fffffff;
 
 template <int D>
 struct WtShape {
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
   uint64_t* pv_done = p_half + 2;  // [2]
   uint64_t* s_free = pv_done + 2;  // [2] (kEarly)
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(s_free + 2);
-  uint32_t* dirty = tmem_holder + 1;
+  int* dirty = reinterpret_cast<int*>(tmem_holder + 1);  // kWtClean, or the first key of the first marked V tile
 
   pdl_trigger();
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       mbar_init(&pv_done[i], 1);
       mbar_init(&s_free[i], 4);
     }
-    *dirty = 0;
+    *dirty = kWtClean;
     mbar_fence_init();
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
   float* part_o = reinterpret_cast<float*>(ring);
   float* part_m = part_o + splits * share * D;
   float* part_l = part_m + splits * share;
-  uint32_t* part_mark = reinterpret_cast<uint32_t*>(part_l + splits * share);
+  int* part_mark = reinterpret_cast<int*>(part_l + splits * share);
   static_assert((2 * kWtRows + kWinSplits) * (D + 2) * 4 + kWinSplits * 4 <= kStages * S::kTile,
                 "the ring holds a CTA's share of all parts");
   float m = -INFINITY, l = 0.0f;  // of a softmax thread's row
@@ -358,7 +359,9 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       // A V tile that some query does not see whole is looked over before the MMAs may have it:
       // rows that no query of this CTA sees (ends of pages, tokens before the window) are zeroed, since
       // their weights are 0 but 0 * NaN is not; an infinity or NaN in a row that only some queries
-      // see marks the CTA, whose rows are then computed one by one (window_row).
+      // see marks the CTA with the tile's first key (the first such tile's, as keys go up).  A query tile
+      // that sees as far computes its rows one by one (window_row); one that ends before must not depend
+      // on whether this warp is ahead of it.
       bool ok = true;
       for (int j = 0; j < n && ok; ++j) {
         const int st = kSK + j % kSV;
@@ -388,7 +391,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
                 bad |= nonfinite2<T>(x[u].x) | nonfinite2<T>(x[u].y) | nonfinite2<T>(x[u].z) | nonfinite2<T>(x[u].w);
             }
           }
-          if (bad) *dirty = 1;
+          if (bad && *reinterpret_cast<volatile int*>(dirty) == kWtClean) *dirty = k0;
           fence_async_smem_cta();
         }
         __syncwarp();
@@ -687,10 +690,10 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       if (ok && np > 0) ok = mbar_wait(&pv_done[i], (np - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      // warp 11's mark: every tile it looked at was multiplied before pv_done
+      // warp 11's mark: its tiles up to this query tile's last were looked at before pv_done
       if (splits > 1) {
         // joined below
-      } else if (ok && *reinterpret_cast<volatile uint32_t*>(dirty)) {
+      } else if (ok && *reinterpret_cast<volatile int*>(dirty) < mine.hi.end) {
         for (int x = 0; x < 32; ++x) {
           const int rr = row0 + i * kWtRows + quarter * 32 + x;
           if (rr < row1) window_row<T, D>(a, b, seq, a.by_group.div(rr), kvh * a.group + a.by_group.mod(rr), lane);
@@ -757,7 +760,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         st_cluster(mapa_shared(smem_u32(part_l + slot), owner), l);
       }
       if (threadIdx.x < splits)
-        st_cluster(mapa_shared(smem_u32(part_mark + rank), threadIdx.x), __uint_as_float(*reinterpret_cast<volatile uint32_t*>(dirty)));
+        st_cluster(mapa_shared(smem_u32(part_mark + rank), threadIdx.x), __int_as_float(*reinterpret_cast<volatile int*>(dirty)));
       const uint32_t dst = mapa_shared(smem_u32(part_o + slot * D), owner);
 #pragma unroll 1
       for (int c = 0; np > 0 && c < D / 32; ++c) {
@@ -773,8 +776,8 @@ __global__ void __launch_bounds__(kWtThreads, 1)
     cluster_sync_all();
     const int own0 = rank * share, own = min(share, row1 - row0 - own0);  // this CTA's rows
     if (warp < 8 && own > 0) {
-      uint32_t marked = 0;
-      for (int x = 0; x < splits; ++x) marked |= part_mark[x];
+      bool marked = false;
+      for (int x = 0; x < splits; ++x) marked |= part_mark[x] != kWtClean;
       if (marked) {
         for (int r = row0 + own0 + warp; r < row0 + own0 + own; r += 8)
           window_row<T, D>(a, b, seq, a.by_group.div(r), kvh * a.group + a.by_group.mod(r), lane);

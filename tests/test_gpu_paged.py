@@ -817,3 +817,24 @@ def test_outputs_that_overlap_other_tensors_are_refused(pkg, cuda):
     want = pkg.qk_norm_rope(x, k, pos, f, axes=(64,))  # in place among the columns of one projection
     got = pkg.qk_norm_rope(x, k, pos, f, axes=(64,), q_out=x, k_out=k)
     assert all(torch.equal(a, b) for a, b in zip(want, got)) and got[0] is x and got[1] is k
+
+
+@pytest.mark.parametrize("d,dtype", [(64, BF), (64, HF), (128, BF)])
+def test_attn_window_with_non_finite_values_is_reproducible(pkg, cuda, d, dtype):
+    """Prompts whose second 128 rows see an infinity in part, which the first 128 do not see: the same bits every
+    time, and right ones."""
+    n = 80  # enough sequences that no cluster shares the keys of one
+    q, kp, vp, table, lens, cu = attn_inputs(cuda, [256] * n, [256] * n, 2, 2, d, dtype, 16)
+    for b in range(n):  # token 250 in one head, an early one (seen by all rows after it) in the other
+        vp[int(table[b, 15]), 0, 10, 3] = math.inf
+        vp[int(table[b, 0]), 1, 5 + b % 8, 7] = -math.inf
+    want = pkg.attn_window(q, kp, vp, table, lens, cu, max_q=256)
+    for _ in range(20):
+        assert torch.equal(pkg.attn_window(q, kp, vp, table, lens, cu, max_q=256).view(torch.int16),
+                           want.view(torch.int16))
+    for b in (0, n - 1):
+        rows = slice(256 * b, 256 * (b + 1))
+        ref = attn_ref(q[rows], kp, vp, table[b: b + 1], lens[b: b + 1], [0, 256], None, 0, 1, d ** -0.5)
+        fine = ref[0].isfinite()
+        check(want[rows][fine], ref[0][fine], attn_tol(ref, dtype, d)[fine])
+        assert (want[rows][250:, 0, 3] == math.inf).all() and want[rows][:250, 0, 3].isfinite().all()
