@@ -11,8 +11,9 @@
 // P = exp2(S * scale - m) and writes it in 16 bits over S, O_i += P_i V_j (P from TMEM).  The MMA warp
 // alternates PV_0(j), QK_0(j+1), PV_1(j), QK_1(j+1): while one tile's softmax runs, the tensor
 // cores work for the other.  At D = 64 there is room for P beside S, and S_i(j+1) is computed while
-// softmax i works on tile j.  m is the running maximum, moved (and O rescaled) only when it
-// grows by more than 2^8, which keeps every p below 2^8 and the sum exact to fp32.
+// softmax i works on tile j.  m is the running maximum (Milakov and Gimelshein, "Online normalizer
+// calculation for softmax", 2018), moved (and O rescaled) only when it grows by more than 2^8, which keeps
+// every p below 2^8 and the sum exact to fp32.
 #pragma once
 
 namespace oasis {
@@ -35,7 +36,7 @@ struct WtShape {
   // D = 64 leaves TMEM columns for P beside S: the next S is then computed under the softmax
   static constexpr bool kEarly = D == 64;
   // quarters of P that the MMAs get before the rest is there: with two or three, 384 or 399 us for a
-  // prompt of 8,191 tokens at D = 128, 77 or 71 us for 8 sessions' frames at D = 64
+  // prompt of 8,191 tokens at D = 128 (short bursts; sustained 439), 77 or 71 us for 8 sessions' frames at D = 64
   static constexpr int kHandover = kEarly ? 3 : 2;
   // registers of a softmax and of a helping thread: the prompt takes 390 us with 208 and 88, 8 sessions'
   // frames 80 (the compiler orders the softmax by what it has)

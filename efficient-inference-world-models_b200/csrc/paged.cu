@@ -28,7 +28,7 @@ int pages_check(const oasis_pages_t* p, const char* who) {
 // contiguous run; it is cut into pieces of kCopyPiece bytes, one per CTA.  CTAs of the same
 // piece of successive pairs are neighbours, so a source copied to several forks comes from
 // L2 after its first read.  Bound by HBM, every byte read once and written once: 1,500 pages of 16
-// layers (3.1 GB) take 467 us, 6.7 TB/s; one page of 16 layers (2 MB) 2.4 us.
+// layers (3.1 GB) take 467 us, 6.7 TB/s; one page of 16 layers (2 MB) 2.0 us.
 // The pointers are not __restrict__: that would let the sources be read through the read-only path, and
 // with dependent launches the kernel that appends to the pages may still run when this one starts.
 // ----------------------------------------------------------------------------------

@@ -403,7 +403,7 @@ def attn_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, p
     the first ``sinks``.  ``scale`` defaults to head_dim ** -0.5.  A query that sees nothing gets zeros.
 
     ``max_q`` / ``max_kv`` (bounds on the queries and tokens of a sequence) only choose the launch; too
-    small ones cost time.
+    small ones cost time, and so does a missing ``max_q`` of a batch (all queries count as one sequence's).
     Rows that belong to no sequence are not written.  ``out`` may be q, and otherwise overlaps no tensor of the
     call.  Returns out, or (out, lse)
     with lse fp32 [tokens][heads], the natural logarithm of the softmax sum."""

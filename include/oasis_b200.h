@@ -368,7 +368,8 @@ int oasis_pages_copy(const oasis_pages_t* src, const oasis_pages_t* dst, const i
  * Pair p is dims (2p, 2p+1) if `interleaved`, else (p, p + rot/2) with rot = sum(axis_dims);
  * axis a owns axis_dims[a]/2 consecutive pairs.
  * Strides are in elements; the head_dim elements of a head are contiguous.  Bases are 16-byte
- * aligned, strides multiples of 16 bytes.  q_out may be q and k_out may be k (same strides).
+ * aligned, strides multiples of 16 bytes.  q_out may be q and k_out may be k (same strides); otherwise
+ * the outputs overlap no other tensor of the call.
  * With `pages` (one layer: the slice of it) k and v of token i go into slot slots[i] = page *
  * page_tokens + offset instead of k_out; tokens whose slot is outside the pages are not stored.
  * head_dim 32, 64, 128 or 256; the half-split form needs rot % 16 == 0. */
@@ -401,7 +402,8 @@ int oasis_qk_norm_rope(const oasis_qk_norm_rope_t* args, cudaStream_t stream);
  * A query that sees nothing gets zeros (lse: -inf).  Rows outside every sequence are not
  * written.  out may be q (same strides).  lse (may be NULL): fp32 [tokens][heads], natural
  * logarithm.  Keys and values that a query does not see do not reach its result, whatever
- * they hold.
+ * they hold.  An infinite value that it sees gives infinity or, under a weight that vanishes in
+ * the pages' type, NaN.
  * heads % kv_heads == 0; head_dim 64 or 128; page_tokens % 16 == 0; bf16 or fp16.
  * kv_len is cut to what the table holds, cu_q to the rows there are.  max_q and max_kv are bounds
  * for choosing the launch (0: from the shapes); they do not change the result, but bounds that
